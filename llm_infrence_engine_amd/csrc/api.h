@@ -236,6 +236,34 @@ long long ms_sample_workspace_bytes(int n_rows);
 int ms_sample(const float* logits, long long ld, int n_rows, int vocab, const float* temperature, const int* top_k,
               const float* top_p, const unsigned long long* seeds, const int* draw_index, int* out, void* workspace,
               int use_top_k, int use_top_p, hipStream_t stream);
+// out [n_rows, vocab] (row stride out_ld): the distributions ms_sample would draw from; arguments and workspace as there.
+// out must not be logits.
+int ms_probabilities(const float* logits, long long ld, int n_rows, int vocab, const float* temperature, const int* top_k,
+                     const float* top_p, float* out, long long out_ld, void* workspace, int use_top_k, int use_top_p,
+                     hipStream_t stream);
+
+// ---- steps that check trees of drafted tokens (csrc/tree_attention.hip, csrc/drafts.hip).
+// Token n, the i-th of request r = token_req[n], sees the entries of r before the step's and of the step's entries those with
+// a bit in its row of tree int32 [n_tokens, words].  context_lens [R]: entries with the step's.
+int ms_tree_attention_generic(const void* q, long long q_stride, const void* k_pages, const void* v_pages, const int* block_table,
+                              int table_stride, const int* table_rows, const int* token_req, const int* q_start,
+                              const int* context_lens, const int* n_live_tokens, const int* tree, int words, void* out,
+                              long long out_stride, int n_tokens, int num_heads, int num_kv_heads, int head_dim, int value_dim,
+                              int page_size, float scale, int v_transposed, int dtype, hipStream_t stream);
+
+// p, q [n_tokens, vocab] (q may be null), tokens / parents / uniforms [n_tokens], q_start [n_requests + 1] -> nodes
+// [n_requests, depth] (the accepted path, -1 behind it), counts [n_requests], out [n_requests] (the token drawn behind it).
+int ms_verify_drafts(const float* p, const float* q, int n_tokens, int vocab, const int* tokens, const int* parents,
+                     const int* q_start, const float* uniforms, int n_requests, int* nodes, int depth, int* counts, int* out,
+                     hipStream_t stream);
+
+// pages / heads / widths / transposed: host arrays of n_tensors (at most ms_keep_tokens_max()); pages[i] [layers, num_pages,
+// heads[i], page_size, widths[i]], or [.., widths[i], page_size].  Entry first[r] + nodes[r][i] goes to first[r] + i.
+int ms_keep_tokens_max();
+int ms_keep_tokens(void* const* pages, const int* heads, const int* widths, const int* transposed, int n_tensors, int layers,
+                   int num_pages, int page_size, const int* block_table, int table_stride, const int* table_rows,
+                   const int* first, const int* nodes, int depth, const int* counts, int n_requests, int dtype,
+                   hipStream_t stream);
 
 // ---- mixers with a fixed-size state (csrc/sequence.hip).  A step's requests: tokens q_start[r]..q_start[r+1]-1, state
 // slot state_slots[r]; token_req [n_tokens]; n_live_tokens (may be null): tokens from there on belong to no request.

@@ -431,6 +431,45 @@ sample_draw_kernel(const float* __restrict__ logits, size_t ld, int V, const flo
   if (threadIdx.x == 0) out[r] = top.i == 0x7fffffff ? 0 : top.i;
 }
 
+// The distribution the draw is made from: mass / total of what is kept, 0 elsewhere.  A row without temperature, or without
+// any mass (NaN or -inf only), has a one where the greedy choice stands.
+__global__ void __launch_bounds__(THREADS)
+probabilities_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
+                     const RowWork* __restrict__ work, int n_chunks, float* __restrict__ out, size_t out_ld) {
+  __shared__ MaxIdx red_mi[THREADS / MS_WAVE];
+  const int r = blockIdx.y, c = blockIdx.x;
+  const RowWork& w = work[r];
+  const float* row = logits + (size_t)r * ld;
+  float* to = out + (size_t)r * out_ld;
+  int begin, end;
+  chunk_range(V, n_chunks, c, &begin, &end);
+  const float T = temperature[r];
+  int one = -1;
+  unsigned long long total = 0;
+  if (!(T > 0.f)) {
+    MaxIdx top = {-INFINITY, 0x7fffffff};
+    for (int k = 0; k < n_chunks; ++k) top = better(top, MaxIdx{__uint_as_float(w.chunk_max[k]), (int)w.chunk_mass[k]});
+    one = top.i == 0x7fffffff ? 0 : top.i;
+  } else {
+    for (int k = 0; k < n_chunks; ++k) total += w.chunk_mass[k];
+    if (total == 0) {
+      const MaxIdx top = block_argmax(row, 0, V, red_mi);
+      one = top.i == 0x7fffffff ? 0 : top.i;
+    }
+  }
+  if (one >= 0) {
+    for (int i = begin + threadIdx.x; i < end; i += THREADS) to[i] = i == one ? 1.f : 0.f;
+    return;
+  }
+  const unsigned floor_key = w.floor_key;
+  const float inv_t = 1.0f / T, zmax = key_value(row_max_key(w, n_chunks));
+  const float inv = (float)((double)(1ull << FIX_PLACES) / (double)total);
+  for_share(row, begin, end, [&](int i, float v) {
+    const float s = v * inv_t;
+    to[i] = s == s && order_key(s) >= floor_key ? expf(s - zmax) * inv : 0.f;
+  });
+}
+
 // First maximum of a row in two stages, so that a few rows still use the whole chip: stage 1 finds the best
 // of each of n_chunks slices of the row, stage 2 the best of those (larger value, then smaller index).
 __global__ void __launch_bounds__(256)
@@ -545,25 +584,19 @@ extern "C" int ms_argmax_static(const float* logits, long long ld, int n_rows, i
 // Bytes of workspace ms_sample needs for n_rows rows (any contents: the first kernel makes it ready).
 extern "C" long long ms_sample_workspace_bytes(int n_rows) { return (long long)sizeof(RowWork) * (n_rows > 0 ? n_rows : 0); }
 
-// One token per row.  Rows with temperature <= 0 (or a null temperature) take the first maximum.  use_top_k /
-// use_top_p: 0 if no row has a top_k in (0, vocab) / a top_p below 1 (their kernels are then left out; when in
-// doubt pass 1).  workspace: ms_sample_workspace_bytes(n_rows) bytes, 8-byte aligned.
-extern "C" int ms_sample(const float* logits, long long ld, int n_rows, int vocab, const float* temperature,
-                         const int* top_k, const float* top_p, const unsigned long long* seeds,
-                         const int* draw_index, int* out, void* workspace, int use_top_k, int use_top_p,
-                         hipStream_t stream) {
-  if (n_rows <= 0) return MS_OK;
-  if (vocab <= 0 || ld < vocab || n_rows > 65535) return MS_BAD_ARG;
-  if (temperature == nullptr) return MS_BAD_ARG;      // all rows greedy: ms_argmax is the entry for that
-  if (workspace == nullptr || ((uintptr_t)workspace % 8)) return MS_BAD_ARG;
-  RowWork* work = (RowWork*)workspace;
-  // About one block for every CU, but 8 to 24 to a row: every block of a row adds its histogram to the row's with
-  // atomics on the same few bins, and reads the histogram of the level before whole, so more blocks to a row cost
-  // more than they spread (8 rows of 151,936: 113 us with 64 blocks a row, 71 with 24; 64 rows: 141 us with 8,
-  // 179 with 4, 182 with 16).
+// About one block for every CU, but 8 to 24 to a row: every block of a row adds its histogram to the row's with
+// atomics on the same few bins, and reads the histogram of the level before whole, so more blocks to a row cost
+// more than they spread (8 rows of 151,936: 113 us with 64 blocks a row, 71 with 24; 64 rows: 141 us with 8,
+// 179 with 4, 182 with 16).
+static int sample_chunks(int n_rows, int vocab) {
   int n_chunks = ms_compute_units() / n_rows;
   n_chunks = std::max(8, std::min(n_chunks, 24));
-  n_chunks = std::max(1, std::min(std::min(n_chunks, MAX_CHUNKS), (vocab + 2047) / 2048));
+  return std::max(1, std::min(std::min(n_chunks, MAX_CHUNKS), (vocab + 2047) / 2048));
+}
+
+// The kernels up to every chunk's kept mass.
+static void sample_thresholds(const float* logits, long long ld, int n_rows, int vocab, const float* temperature, const int* top_k,
+                              const float* top_p, RowWork* work, int n_chunks, int use_top_k, int use_top_p, hipStream_t stream) {
   const dim3 grid(n_chunks, n_rows), block(THREADS);
   if (top_k == nullptr) use_top_k = 0;
   if (top_p == nullptr) use_top_p = 0;
@@ -580,6 +613,36 @@ extern "C" int ms_sample(const float* logits, long long ld, int n_rows, int voca
       sample_level_kernel<3><<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks, 3);
   }
   sample_chunk_mass_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, use_top_p ? top_p : nullptr, work, n_chunks, thresholds);
-  sample_draw_kernel<<<dim3(n_rows), block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, seeds, draw_index, work, n_chunks, out);
+}
+
+// One token per row.  Rows with temperature <= 0 (or a null temperature) take the first maximum.  use_top_k /
+// use_top_p: 0 if no row has a top_k in (0, vocab) / a top_p below 1 (their kernels are then left out; when in
+// doubt pass 1).  workspace: ms_sample_workspace_bytes(n_rows) bytes, 8-byte aligned.
+extern "C" int ms_sample(const float* logits, long long ld, int n_rows, int vocab, const float* temperature,
+                         const int* top_k, const float* top_p, const unsigned long long* seeds,
+                         const int* draw_index, int* out, void* workspace, int use_top_k, int use_top_p,
+                         hipStream_t stream) {
+  if (n_rows <= 0) return MS_OK;
+  if (vocab <= 0 || ld < vocab || n_rows > 65535) return MS_BAD_ARG;
+  if (temperature == nullptr) return MS_BAD_ARG;      // all rows greedy: ms_argmax is the entry for that
+  if (workspace == nullptr || ((uintptr_t)workspace % 8)) return MS_BAD_ARG;
+  RowWork* work = (RowWork*)workspace;
+  const int n_chunks = sample_chunks(n_rows, vocab);
+  sample_thresholds(logits, ld, n_rows, vocab, temperature, top_k, top_p, work, n_chunks, use_top_k, use_top_p, stream);
+  sample_draw_kernel<<<dim3(n_rows), dim3(THREADS), 0, stream>>>(logits, (size_t)ld, vocab, temperature, seeds, draw_index, work, n_chunks, out);
+  return ms_launch_status();
+}
+
+// out[r, :] = the distribution ms_sample would draw row r's token from; arguments as there.
+extern "C" int ms_probabilities(const float* logits, long long ld, int n_rows, int vocab, const float* temperature,
+                                const int* top_k, const float* top_p, float* out, long long out_ld, void* workspace,
+                                int use_top_k, int use_top_p, hipStream_t stream) {
+  if (n_rows <= 0) return MS_OK;
+  if (vocab <= 0 || ld < vocab || out_ld < vocab || n_rows > 65535 || temperature == nullptr) return MS_BAD_ARG;
+  if (workspace == nullptr || ((uintptr_t)workspace % 8)) return MS_BAD_ARG;
+  RowWork* work = (RowWork*)workspace;
+  const int n_chunks = sample_chunks(n_rows, vocab);
+  sample_thresholds(logits, ld, n_rows, vocab, temperature, top_k, top_p, work, n_chunks, use_top_k, use_top_p, stream);
+  probabilities_kernel<<<dim3(n_chunks, n_rows), dim3(THREADS), 0, stream>>>(logits, (size_t)ld, vocab, temperature, work, n_chunks, out, (size_t)out_ld);
   return ms_launch_status();
 }

@@ -118,6 +118,15 @@ _SIGNATURES = {
     "ms_sample": [_c_ptr, _c_ll, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
                   _c_ptr],
     "ms_sample_workspace_bytes": [_c_int],
+    "ms_probabilities": [_c_ptr, _c_ll, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_int, _c_int, _c_ptr],
+    "ms_tree_attention_generic": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                  _c_int, _c_ptr, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int,
+                                  _c_ptr],
+    "ms_verify_drafts": [_c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr,
+                         _c_ptr],
+    "ms_keep_tokens_max": [],
+    "ms_keep_tokens": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr,
+                       _c_int, _c_ptr, _c_int, _c_int, _c_ptr],
     "ms_short_conv": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_int, _c_int,
                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
     "ms_gated_delta": [_c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_int, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
@@ -1469,6 +1478,195 @@ def paged_attention(q: torch.Tensor, kv, ctx, out: torch.Tensor, num_heads: int,
     return paged_attention_generic(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.positions, out,
                                    num_heads, scale, window, kv.v_transposed, kv.table_rows, ctx.n_live_tokens, sink,
                                    softcap, slopes, gate, out_scale)
+
+
+# ------------------------------------------------------------------------------------------------ trees of drafted tokens
+def _here(*tensors) -> None:
+    """Work goes to the current device's current stream: tensors of another device are refused."""
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"a tensor is on cuda:{t.get_device()}, the current device is cuda:{device}")
+
+
+def probabilities(logits: torch.Tensor, out: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+                  top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                  use_top_k: bool = True, use_top_p: bool = True) -> torch.Tensor:
+    """out[r, :] = the distribution that ``sample`` draws row r's token from: softmax(logits[r] / temperature[r]) over the
+    tokens that top-k and top-p keep, 0 elsewhere; with ``temperature`` <= 0 (or without one) a one at the first maximum.
+    NaN logits get 0; a row without any mass (NaN or -inf only) has its one where the greedy choice stands.  float32
+    [M, V] both, ``out`` another tensor than ``logits``; the other arguments as for ``sample``."""
+    _check(logits, "logits", torch.float32)
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [rows, vocabulary], got {list(logits.shape)}")
+    M, V = logits.shape
+    _check(out, "out", torch.float32, (M, V))
+    if M > 65535:
+        raise ValueError("at most 65,535 rows to a call")
+    if M == 0 or V == 0:
+        return out
+    if out.data_ptr() < logits.data_ptr() + logits.nbytes and logits.data_ptr() < out.data_ptr() + out.nbytes:
+        raise ValueError("out must not share memory with logits")
+    for t, name, dt in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32)):
+        if t is not None:
+            _check(t, name, dt, (M,))
+    _here(logits, out, temperature, top_k, top_p)
+    if temperature is None:
+        temperature = torch.zeros(M, dtype=torch.float32, device=logits.device)
+    work = torch.empty(int(_get("ms_sample_workspace_bytes")(M)), dtype=torch.uint8, device=logits.device)
+    _call("ms_probabilities", logits.data_ptr(), V, M, V, temperature.data_ptr(), _ptr(top_k), _ptr(top_p), out.data_ptr(), V,
+          work.data_ptr(), int(use_top_k and top_k is not None), int(use_top_p and top_p is not None), _stream())
+    return out
+
+
+def _tree_words(tree: torch.Tensor, n_tokens: int, max_q_len: int) -> int:
+    """The words a token has of its mask."""
+    _check(tree, "tree", torch.int32, (n_tokens, None))
+    if tree.shape[1] * 32 < max_q_len or tree.shape[1] == 0:
+        raise ValueError(f"tree has {tree.shape[1]} words of 32 bits a token for trees of up to {max_q_len} tokens")
+    return tree.shape[1]
+
+
+def tree_attention_generic(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                           token_req: torch.Tensor, q_start: torch.Tensor, context_lens: torch.Tensor, tree: torch.Tensor,
+                           out: torch.Tensor, num_heads: int, scale: float, max_q_len: int, v_transposed: bool = False,
+                           table_rows: Optional[torch.Tensor] = None, n_live_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``tree_attention`` on the vector ALUs: float32 or bfloat16, keys and values of any size up to 256, pages of any size.
+    Tensors as for ``paged_attention_generic``, q_start int32 [R + 1], context_lens int32 [R]."""
+    _check(k_pages, "k_pages")
+    P, nkv, page_size, d = k_pages.shape
+    _check(v_pages, "v_pages", k_pages.dtype, (P, nkv, None, None))
+    dv = v_pages.shape[2] if v_transposed else v_pages.shape[3]
+    _check(v_pages, "v_pages", k_pages.dtype, _v_shape(k_pages, v_transposed, dv))
+    q_stride = _tree_step(q, k_pages, block_table, q_start, context_lens, table_rows, out, num_heads, nkv, d, dv, max_q_len)
+    N = q.shape[0]
+    words = _tree_words(tree, N, max_q_len)
+    _check(token_req, "token_req", torch.int32, (N,))
+    if n_live_tokens is not None:
+        _check(n_live_tokens, "n_live_tokens", torch.int32, (1,))
+    _here(q, k_pages, v_pages, block_table, table_rows, token_req, q_start, context_lens, n_live_tokens, tree, out)
+    _call("ms_tree_attention_generic", q.data_ptr(), q_stride, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
+          block_table.shape[1], _ptr(table_rows), token_req.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(),
+          _ptr(n_live_tokens), tree.data_ptr(), words, out.data_ptr(), num_heads * dv, N, num_heads, nkv, d, dv, page_size,
+          float(scale), int(v_transposed), _code(q.dtype), _stream())
+    return out
+
+
+def _tree_step(q, k_pages, block_table, q_start, context_lens, table_rows, out, num_heads, nkv, d, dv, max_q_len) -> int:
+    """Checks what the kernels of ``tree_attention`` have in common; the stride of q's rows."""
+    stride = _rows2d(q, "q", k_pages.dtype)
+    N = q.shape[0]
+    if q.shape[1] < num_heads * d:
+        raise ValueError(f"q must be [N, >= {num_heads * d}], got {list(q.shape)}")
+    if num_heads <= 0 or num_heads % nkv:
+        raise ValueError(f"{num_heads} query heads cannot share {nkv} key/value heads")
+    _check(out, "out", k_pages.dtype, (N, num_heads * dv))
+    _check(block_table, "block_table", torch.int32, (None, None))
+    _check(context_lens, "context_lens", torch.int32, (None,))
+    R = context_lens.numel()
+    _check(q_start, "q_start", torch.int32, (R + 1,))
+    if table_rows is not None:
+        _check(table_rows, "table_rows", torch.int32, (R,))
+    elif block_table.shape[0] < R:
+        raise ValueError(f"the block table has {block_table.shape[0]} rows for {R} requests")
+    if max_q_len < 1:
+        raise ValueError(f"max_q_len {max_q_len}: a tree has at least one token")
+    return stride
+
+
+def tree_attention(q: torch.Tensor, kv, ctx, tree: torch.Tensor, out: torch.Tensor, num_heads: int, scale: float) -> torch.Tensor:
+    """Attention of a step whose requests check trees of drafted tokens (``ctx``: its StepContext, ``kv``: the run's
+    KVView).  A token sees its request's entries from before the step, whatever its position, and of the step's own tokens
+    those in its row of ``tree``, int32 [N, words]: bit j % 32 of word j / 32 stands for the request's j-th token of the
+    step (its ancestors and itself, as a rule; bits behind the tree are ignored).  A token that sees nothing gets zeros.
+    The step's keys and values lie in the cache in the order of the tokens (``slot_mapping``), encoded with whatever
+    positions the tree gives them; ``keep_tokens`` moves together what is accepted."""
+    d, page_size = kv.k_pages.shape[3], kv.k_pages.shape[2]
+    return tree_attention_generic(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.q_start, ctx.context_lens, tree,
+                                  out, num_heads, scale, max(1, ctx.max_q_len), kv.v_transposed, kv.table_rows, ctx.n_live_tokens)
+
+
+def verify_drafts(p: torch.Tensor, q: Optional[torch.Tensor], token_ids: torch.Tensor, parents: torch.Tensor,
+                  q_start: torch.Tensor, uniforms: torch.Tensor, nodes: torch.Tensor, counts: torch.Tensor,
+                  out: torch.Tensor) -> torch.Tensor:
+    """Accepts drafted tokens so that every token is distributed as if it had been drawn from the target one at a time.
+
+    Request r owns the rows q_start[r] .. q_start[r + 1] - 1 of a step: the first is its last token (the root), the others
+    are guesses, each behind its parent: ``parents`` int32 [N], the parent's index among the request's rows, below the
+    row's own (-1 for the root).  Row n of ``p`` float32 [N, V] is the target's distribution behind token n
+    (``probabilities``), row n of ``q`` the one its children were drawn from, each by itself; without ``q`` the guesses are
+    taken as they are.  ``uniforms`` float32 [N] in [0, 1): a guess's number decides about it, the root's draws the token
+    behind the accepted path.  Guesses outside the vocabulary are passed over.
+
+    nodes[r] int32 [R, depth]: the accepted path's rows, 0 first, then -1; a path that fills it ends there.  counts[r]: its
+    length.  out[r]: the token drawn behind it.  A request without rows gets -1, 0 and -1."""
+    _check(p, "p", torch.float32, (None, None))
+    N, V = p.shape
+    if V == 0:
+        raise ValueError("p has no vocabulary")
+    if q is not None:
+        _check(q, "q", torch.float32, (N, V))
+    _check(token_ids, "token_ids", torch.int32, (N,))
+    _check(parents, "parents", torch.int32, (N,))
+    _check(uniforms, "uniforms", torch.float32, (N,))
+    _check(q_start, "q_start", torch.int32, (None,))
+    R = q_start.numel() - 1
+    if R < 0 or R > 65535:
+        raise ValueError("q_start has one number more than there are requests, at most 65,536")
+    _check(nodes, "nodes", torch.int32, (R, None))
+    if nodes.shape[1] < 1:
+        raise ValueError("nodes must have room for the root")
+    _check(counts, "counts", torch.int32, (R,))
+    _check(out, "out", torch.int32, (R,))
+    _here(p, q, token_ids, parents, q_start, uniforms, nodes, counts, out)
+    _call("ms_verify_drafts", p.data_ptr(), _ptr(q), N, V, token_ids.data_ptr(), parents.data_ptr(), q_start.data_ptr(),
+          uniforms.data_ptr(), R, nodes.data_ptr(), nodes.shape[1], counts.data_ptr(), out.data_ptr(), _stream())
+    return out
+
+
+def keep_tokens(pages, transposed, block_table: torch.Tensor, first: torch.Tensor, nodes: torch.Tensor, counts: torch.Tensor,
+                table_rows: Optional[torch.Tensor] = None) -> None:
+    """Moves what an accepted path stored together: entry first[r] + nodes[r, i] of request r becomes entry first[r] + i, for
+    i < counts[r], in every layer and head of every tensor of ``pages``: [layers, pages, heads, page_size, width] each, or
+    [layers, pages, heads, width, page_size] where ``transposed`` says so (or without the layers).  ``first`` int32 [R]: the
+    entry of the step's first token (context length less tokens); ``nodes`` int32 [R, depth] and ``counts`` int32 [R] as
+    ``verify_drafts`` leaves them: increasing, 0 first.  Entries whose page is the null page or outside the pool stay."""
+    pages, transposed = list(pages), list(transposed)
+    if not pages or len(pages) != len(transposed):
+        raise ValueError("one or more page tensors, and for each whether it is transposed")
+    most = _get("ms_keep_tokens_max")()
+    if len(pages) > most:
+        raise ValueError(f"at most {most} page tensors to a call")
+    _check(nodes, "nodes", torch.int32, (None, None))
+    R, depth = nodes.shape
+    _check(first, "first", torch.int32, (R,))
+    _check(counts, "counts", torch.int32, (R,))
+    _check(block_table, "block_table", torch.int32, (None, None))
+    if table_rows is not None:
+        _check(table_rows, "table_rows", torch.int32, (R,))
+    elif block_table.shape[0] < R:
+        raise ValueError(f"the block table has {block_table.shape[0]} rows for {R} requests")
+    sizes = []
+    for t, flip in zip(pages, transposed):
+        _check(t, "pages", pages[0].dtype)
+        if t.dim() not in (4, 5):
+            raise ValueError(f"pages must be [layers, pages, heads, page size, width] or without the layers, got {list(t.shape)}")
+        L, P, heads, a, b = t.shape if t.dim() == 5 else (1, *t.shape)
+        sizes.append((L, P, b if flip else a, heads, a if flip else b))
+    if any(s[:3] != sizes[0][:3] for s in sizes):
+        raise ValueError("the page tensors of a call have the same layers, pages and page size")
+    L, P, page_size = sizes[0][:3]
+    code = _code(pages[0].dtype)
+    if R == 0 or depth == 0 or L == 0 or P == 0:
+        return
+    if R > 65535:
+        raise ValueError("at most 65,535 requests to a call")
+    _here(*pages, block_table, first, nodes, counts, table_rows)
+    keep, ptrs = _pointer_array(pages)
+    n = len(pages)
+    ints = [(_c_int * n)(*v) for v in ([s[3] for s in sizes], [s[4] for s in sizes], [int(bool(f)) for f in transposed])]
+    _call("ms_keep_tokens", ptrs, *(ctypes.cast(a, ctypes.c_void_p) for a in ints), n, L, P, page_size, block_table.data_ptr(),
+          block_table.shape[1], _ptr(table_rows), first.data_ptr(), nodes.data_ptr(), depth, counts.data_ptr(), R, code, _stream())
 
 
 # ------------------------------------------------------------------------------------------------ state-carrying mixers
