@@ -1,0 +1,506 @@
+// The attention of csrc/tree_attention.hip on the matrix cores (v_mfma_f32_16x16x32_bf16), bfloat16 in, float softmax.
+//
+// A column is a (token, query head of the group) pair; a block owns COLS columns of one (request, key/value head) and a share
+// of the request's keys, so a key that is brought in serves all of them.  Its waves are KG groups of WC: the waves of a group
+// own neighbouring columns, NT tiles of 16 each, and walk the same keys, a tile of KEYS at a time, which go from the pages
+// straight to LDS (global_load_lds) one tile ahead; the groups take the tiles in turn and merge at the end.  Products and the
+// layout of LDS are those of csrc/attention_prompt.hip:
+//
+//   S^T[key, col] = K[key, :] . Q^T[:, col],   O^T[dim, col] += V^T[dim, key] . P^T[key, col]
+//
+// where row r of the u-th score product of a unit of 32 keys is its key 8 (r / 4) + 4 u + r % 4, so that a lane (quarter kq)
+// holds the scores of the keys 8 kq .. + 7 and needs one 16-byte read of a value's row.  Keys from before the step are visible
+// to every column; only units that reach into the step's own entries (the last ones) look at the mask.
+// The keys of a request are shared out over n_splits blocks, which leave unnormalised float results that a second kernel
+// adds up: with few columns there is one (request, head) tile for a handful of CUs, and a step waits for the longest chain.
+#include "attention_tiles.h"
+#include "api.h"
+#include <algorithm>
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+constexpr int MAX_SPLITS = 128;
+
+template <int D> __device__ __forceinline__ int permute(int key) {     // where a key's 16-byte pieces lie, by its number in its unit
+  return D == 128 ? (key & 3) | ((key >> 1) & 12) : D == 64 ? ((key >> 1) & 1) | ((key >> 2) & 6) : (key >> 3) & 3;
+}
+
+// The maximum over the four lanes, 16 apart, that share a column.
+__device__ __forceinline__ float column_max(float x) {
+  const unsigned u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const unsigned w = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Which of the n_splits shares of a request's tiles of keys a block has; the shares are even, the last ones may be empty.
+__device__ __forceinline__ int tiles_a_split(int context, int keys, int n_splits) {
+  return ((context + keys - 1) / keys + n_splits - 1) / n_splits;
+}
+
+template <int D, int WC, int KG, int NT>
+struct Shape {
+  static constexpr int COLS = WC * NT * 16, KEYS = WC == 4 ? 64 : 32, CHUNKS = KEYS / 16;
+  static constexpr int CHUNK = 16 * D;                 // values of a chunk of 16 keys, of keys as of values
+  static constexpr int STAGE = 2 * CHUNKS * CHUNK;     // a tile: its chunks of keys, then those of values
+  static constexpr size_t LDS = (size_t)KG * 2 * STAGE * 2;
+};
+
+template <int D, int WC, int KG, int NT>
+__global__ void __launch_bounds__(KG * WC * MS_WAVE, D == 128 ? 2 : 4)
+tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf16* __restrict__ k_pages,
+                           const bf16* __restrict__ vt_pages, const int* __restrict__ block_table, int table_stride,
+                           const int* __restrict__ table_rows, const int* __restrict__ q_start,
+                           const int* __restrict__ context_lens, const unsigned* __restrict__ tree, int words,
+                           bf16* __restrict__ out, size_t out_stride, float* __restrict__ part_o, float* __restrict__ part_ml,
+                           int nh, int nkv, int page_size, float scale_log2e, int n_requests, int n_splits) {
+  typedef Shape<D, WC, KG, NT> S;
+  constexpr int COLS = S::COLS, KEYS = S::KEYS, CHUNKS = S::CHUNKS, CHUNK = S::CHUNK, STAGE = S::STAGE;
+  constexpr int CT = D / 16, PIECES = D / 8, LOADS = CHUNK * 2 / 1024, MINE = CHUNKS / WC;      // chunks a wave brings
+  extern __shared__ __align__(16) unsigned char lds_raw[];
+  bf16* lds = reinterpret_cast<bf16*>(lds_raw);       // [KG][2 tiles][STAGE]
+  const int lane = threadIdx.x & (MS_WAVE - 1);
+  const int kg = __builtin_amdgcn_readfirstlane(threadIdx.x / (WC * MS_WAVE));
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / MS_WAVE) - kg * WC;   // in its group
+  const int col16 = lane & 15, kq = lane >> 4;
+  const int g = blockIdx.x, rep = nh / nkv, split = blockIdx.z;
+
+  int r, tile, n_tiles;
+  find_tile(q_start, n_requests, rep, COLS, blockIdx.y, lane, r, tile, n_tiles);
+  if (r < 0) return;
+  const int* table = block_table + (size_t)(table_rows ? table_rows[r] : r) * table_stride;
+  const int q0 = q_start[r], qlen = q_start[r + 1] - q0, context = context_lens[r], before = context - qlen, ncols = qlen * rep;
+  const int per = tiles_a_split(context, KEYS, n_splits);
+  const int t_begin = split * per, t_end = min((context + KEYS - 1) / KEYS, t_begin + per);
+  if (t_begin >= t_end) return;
+  const int c0 = (tile * WC + wave) * NT * 16;
+  const bool works = c0 < ncols;       // without columns a wave still brings its chunks
+
+  // ---- bringing a tile: the wave's chunks of keys and of values
+  int k_src[MINE][LOADS], v_src[LOADS];                        // what a lane asks for, from the chunk's first value in the page
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int at = j * 512 + lane * 8, key = at / D, piece = (at % D) / 8;
+#pragma unroll
+    for (int b = 0; b < MINE; ++b) k_src[b][j] = key * D + (piece ^ permute<D>(((wave * MINE + b) & 1) * 16 + key)) * 8;
+    const int dim = at / 16, half = (at >> 3) & 1;
+    v_src[j] = dim * page_size + (half ^ ((dim >> 3) & 1)) * 8;
+  }
+  auto page_of = [&](int t, int b) {        // the page of one of the wave's chunks of tile t; past the context: the null page
+    const int key = t * KEYS + (wave * MINE + b) * 16;
+    return key < context ? __builtin_amdgcn_readfirstlane(table[key / page_size]) : 0;
+  };
+  auto bring = [&](int t, const int* pages, int stage) {
+#pragma unroll
+    for (int b = 0; b < MINE; ++b) {
+      const int off = (t * KEYS + (wave * MINE + b) * 16) % page_size;
+      const size_t head = ((size_t)pages[b] * nkv + g) * page_size * D;
+      const bf16* kp = k_pages + head + (size_t)off * D;
+      const bf16* vp = vt_pages + head + off;
+      bf16* to = lds + (kg * 2 + stage) * STAGE + (wave * MINE + b) * CHUNK;
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) __builtin_amdgcn_global_load_lds((global_void*)(kp + k_src[b][j]), (lds_void*)(to + j * 512), 16, 0, 0);
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) __builtin_amdgcn_global_load_lds((global_void*)(vp + v_src[j]), (lds_void*)(to + CHUNKS * CHUNK + j * 512), 16, 0, 0);
+    }
+  };
+  int pages[MINE];
+  if (t_begin + kg < t_end) {
+#pragma unroll
+    for (int b = 0; b < MINE; ++b) pages[b] = page_of(t_begin + kg, b);
+    bring(t_begin + kg, pages, 0);
+  }
+  if (t_begin + kg + KG < t_end) {
+#pragma unroll
+    for (int b = 0; b < MINE; ++b) pages[b] = page_of(t_begin + kg + KG, b);
+  }
+
+  // ---- this lane's columns
+  bool idle[NT];
+  const unsigned* mask[NT];
+  unsigned first_words[NT][2];         // (most trees have no more)
+  bf16x8 qv[NT][D / 32];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int c = c0 + t * 16 + col16, cc = min(c, ncols - 1), tok = q0 + cc / rep;
+    idle[t] = c >= ncols;
+    mask[t] = tree + (size_t)tok * words;
+    first_words[t][0] = mask[t][0];
+    first_words[t][1] = words > 1 ? mask[t][1] : 0u;
+    const bf16* qp = q + (size_t)tok * q_stride + (size_t)(g * rep + cc % rep) * D + kq * 8;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) qv[t][s] = *reinterpret_cast<const bf16x8*>(qp + s * 32);
+  }
+  // which of the keys base + kq * 8 + (0..7) column tile t sees, a bit each
+  auto visible = [&](int t, int base) -> unsigned {
+    const int rel = base + kq * 8 - before;            // the first one's number in the step; below 0: from before
+    if (idle[t]) return 0u;
+    if (rel <= -8) return 0xffu;
+    const int at = max(rel, 0), w = at >> 5;
+    auto word = [&](int i) -> unsigned { return i == 0 ? first_words[t][0] : i == 1 ? first_words[t][1] : i < words ? mask[t][i] : 0u; };
+    unsigned bits = (unsigned)((((unsigned long long)word(w + 1) << 32) | word(w)) >> (at & 31)) & 0xffu;
+    if (rel < 0) bits = ((bits << -rel) | ((1u << -rel) - 1u)) & 0xffu;
+    const int left = qlen - rel;
+    return left >= 8 ? bits : left <= 0 ? 0u : bits & ((1u << left) - 1u);
+  };
+
+  // The sums of the exponentials are those of the rounded ones that meet the values: one more product, of P^T with ones.
+  float m[NT];
+  f32x4 o[CT][NT] = {}, lsum[NT] = {};
+#pragma unroll
+  for (int t = 0; t < NT; ++t) m[t] = -INFINITY;
+  bf16x8 ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.0f;
+
+  int k_row[2], k_perm[2];             // where a lane's fragments lie: key rows of the u-th product of a unit ..
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int key = (col16 >> 2) * 8 + u * 4 + (col16 & 3);
+    k_row[u] = (key >> 4) * CHUNK + (key & 15) * D;
+    k_perm[u] = permute<D>(key);
+  }
+  const int v_row = CHUNKS * CHUNK + (kq >> 1) * CHUNK + col16 * 16 + (((kq & 1) ^ (col16 >> 3)) * 8);     // .. and of 16 dims' values
+
+  // the queries have arrived (said here, where the compiler sees it: otherwise it waits for them, and with them for the
+  // loads to LDS, before the first product of every turn)
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  const int turns = (t_end - t_begin + KG - 1) / KG;
+  for (int turn = 0; turn < turns; ++turn) {
+    const int t = t_begin + turn * KG + kg, stage = turn & 1;
+    // This tile has landed (vmcnt), and the wave's reads of the one before it have ended (lgkmcnt), so that its place may
+    // be filled again.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + KG < t_end) {
+      bring(t + KG, pages, stage ^ 1);
+      if (t + 2 * KG < t_end) {
+#pragma unroll
+        for (int b = 0; b < MINE; ++b) pages[b] = page_of(t + 2 * KG, b);
+      }
+    }
+    if (!works || t >= t_end) continue;      // the same for the whole wave
+#pragma unroll
+    for (int unit = 0; unit < KEYS / 32; ++unit) {
+      const int base = t * KEYS + unit * 32;
+      if (base >= context) break;
+      const bf16* st = lds + (kg * 2 + stage) * STAGE + unit * 2 * CHUNK;
+
+      // scores: s[u][t] holds keys base + kq*8 + u*4 + (0..3) of column t*16 + col16
+      f32x4 s[2][NT];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int t2 = 0; t2 < NT; ++t2) s[u][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) {
+          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(st + k_row[u] + (((ks * 4 + kq) ^ k_perm[u]) & (PIECES - 1)) * 8);
+#pragma unroll
+          for (int t2 = 0; t2 < NT; ++t2) s[u][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qv[t2][ks], s[u][t2], 0, 0, 0);
+        }
+      }
+      const bool masked = base + 31 >= before;     // reaches into the step's own entries, or behind them
+      unsigned sees[NT];
+      if (masked) {
+#pragma unroll
+        for (int t2 = 0; t2 < NT; ++t2) {
+          sees[t2] = visible(t2, base);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!((sees[t2] >> (u * 4 + i)) & 1u)) s[u][t2][i] = -INFINITY;
+        }
+      }
+      // m is the reference of the exponents: it follows the maximum when that has run ahead by REF_SLACK
+      float bmax[NT];
+      bool ahead = false;
+#pragma unroll
+      for (int t2 = 0; t2 < NT; ++t2) {
+        float bm = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bm = fmaxf(bm, s[u][t2][i]);
+        bmax[t2] = bm;
+        ahead |= bm * scale_log2e > m[t2] + REF_SLACK;
+      }
+      if (__builtin_amdgcn_ballot_w64(ahead) != 0) {
+#pragma unroll
+        for (int t2 = 0; t2 < NT; ++t2) {
+          const float bm = column_max(bmax[t2]) * scale_log2e;
+          const bool step = bm > m[t2] + REF_SLACK;
+          const float corr = step ? fast_exp2(m[t2] - bm) : 1.0f;      // m = -inf: 0
+          if (step) m[t2] = bm;
+          lsum[t2] *= corr;
+#pragma unroll
+          for (int c = 0; c < CT; ++c) o[c][t2] *= corr;
+        }
+      }
+      bf16x8 p[NT];
+#pragma unroll
+      for (int t2 = 0; t2 < NT; ++t2) {
+        const float ref = m[t2] == -INFINITY ? 0.f : m[t2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[t2][u * 4 + i] = (__bf16)fast_exp2(fmaf(s[u][t2][i], scale_log2e, -ref));
+        lsum[t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[t2], lsum[t2], 0, 0, 0);
+      }
+      bool spoiled = false;      // some value of the step's own entries that is not finite
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        bf16x8 v = *reinterpret_cast<const bf16x8*>(st + v_row + c * 256);
+        if (masked) {
+          // Values behind the context may be anything a reused page still holds: zeros.  Those of the step's entries that are
+          // not finite would reach columns that do not see them: zeros here, and added below for those that do.
+          u16x8 raw = __builtin_bit_cast(u16x8, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = base + kq * 8 + i;
+            const bool wild = key >= before && (raw[i] & 0x7f80) == 0x7f80;
+            spoiled |= wild && key < context;
+            if (wild || key >= context) raw[i] = 0;
+          }
+          v = __builtin_bit_cast(bf16x8, raw);
+        }
+#pragma unroll
+        for (int t2 = 0; t2 < NT; ++t2) o[c][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t2], o[c][t2], 0, 0, 0);
+      }
+      if (masked && __builtin_amdgcn_ballot_w64(spoiled) != 0) {
+        for (int k = 0; k < 32; ++k) {
+          if (base + k < before || base + k >= context) continue;
+          const int owner = (k >> 3) * 16 + col16;
+#pragma unroll
+          for (int t2 = 0; t2 < NT; ++t2) {
+            float mine = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mine = (k & 7) == i ? (float)p[t2][i] : mine;
+            const float w = __shfl(mine, owner, MS_WAVE);
+            const bool see = (__shfl(sees[t2], owner, MS_WAVE) >> (k & 7)) & 1u;
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int dim = c * 16 + kq * 4 + i;
+                const unsigned short raw = __builtin_bit_cast(unsigned short,
+                    st[CHUNKS * CHUNK + (k >> 4) * CHUNK + dim * 16 + ((((k >> 3) ^ (dim >> 3)) & 1) * 8) + (k & 7)]);
+                if (see && (raw & 0x7f80u) == 0x7f80u) o[c][t2][i] += w * __uint_as_float((unsigned)raw << 16);
+              }
+          }
+        }
+      }
+    }
+  }
+
+  float l[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) l[t] = lsum[t][0];      // every row of the product of ones is the column's sum
+  constexpr int OWN = CT >= KG ? CT / KG : 1;          // tiles of dims a group ends up with
+  if constexpr (KG > 1) {
+    __shared__ float sm_m[KG][COLS], sm_l[KG][COLS];
+    f32x4* sm_o = reinterpret_cast<f32x4*>(lds);       // [group of the sums][wave][tile of dims][NT][64]
+    static_assert((size_t)KG * WC * CT * NT * MS_WAVE * 16 <= S::LDS, "all sums fit");
+    __syncthreads();                                   // nobody reads keys or values any more
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int c = (wave * NT + t) * 16 + col16;
+      if (kq == 0) { sm_m[kg][c] = m[t]; sm_l[kg][c] = l[t]; }
+#pragma unroll
+      for (int d = 0; d < CT; ++d)
+        if (d / OWN != kg) sm_o[(((kg * WC + wave) * CT + d) * NT + t) * MS_WAVE + lane] = o[d][t];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int c = (wave * NT + t) * 16 + col16;
+      float big = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < KG; ++k) big = fmaxf(big, sm_m[k][c]);
+      const float safe = big == -INFINITY ? 0.f : big;
+      l[t] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KG; ++k) l[t] = fmaf(sm_l[k][c], fast_exp2(sm_m[k][c] - safe), l[t]);
+#pragma unroll
+      for (int d = 0; d < CT; ++d) {
+        if (d / OWN != kg) continue;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KG; ++k) {
+          const float f = fast_exp2(sm_m[k][c] - safe);
+          sum += (k == kg ? o[d][t] : sm_o[(((k * WC + wave) * CT + d) * NT + t) * MS_WAVE + lane]) * f;
+        }
+        o[d][t] = sum;
+      }
+      m[t] = big;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (idle[t]) continue;
+    const int c = c0 + t * 16 + col16, tok = q0 + c / rep, head = g * rep + c % rep;
+    if (n_splits > 1) {
+      const size_t slot = ((size_t)tok * nh + head) * n_splits + split;
+#pragma unroll
+      for (int d = 0; d < CT; ++d)
+        if (KG == 1 || d / OWN == kg) *reinterpret_cast<f32x4*>(part_o + slot * D + d * 16 + kq * 4) = o[d][t];
+      if (kq == 0 && kg == 0) { part_ml[slot * 2] = m[t]; part_ml[slot * 2 + 1] = l[t]; }
+    } else {
+      const float inv = l[t] != 0.f ? 1.0f / l[t] : 0.f;      // nothing visible: zeros (a NaN stays one)
+      bf16* op = out + (size_t)tok * out_stride + (size_t)head * D + kq * 4;
+#pragma unroll
+      for (int d = 0; d < CT; ++d) {
+        if (KG > 1 && d / OWN != kg) continue;
+        bf16x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (__bf16)(o[d][t][i] * inv);
+        *reinterpret_cast<bf16x4*>(op + d * 16) = w;
+      }
+    }
+  }
+}
+
+// out[n, h, :] = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the splits that n's request used, a wave to a (token,
+// head): a split's reference and sum to a lane, then every lane its dims of one split after another.
+constexpr int COMBINE_WAVES = 4;
+
+template <int D>
+__global__ void __launch_bounds__(COMBINE_WAVES * MS_WAVE)
+tree_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ token_req,
+                    const int* __restrict__ q_start, const int* __restrict__ context_lens, int n_requests, bf16* __restrict__ out,
+                    size_t out_stride, int n_tokens, int nh, int keys, int n_splits) {
+  constexpr int DL = (D + MS_WAVE - 1) / MS_WAVE;
+  const int lane = threadIdx.x & (MS_WAVE - 1);
+  const long long item = (long long)blockIdx.x * COMBINE_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / MS_WAVE);
+  const int n = (int)(item / nh), h = (int)(item - (long long)n * nh);
+  if (n >= n_tokens || n >= q_start[n_requests]) return;      // (a token that pads a captured batch)
+  const int context = context_lens[token_req[n]];
+  const int per = tiles_a_split(context, keys, n_splits), used = ((context + keys - 1) / keys + per - 1) / per;
+  const size_t slot0 = (size_t)item * n_splits;
+  float m[MAX_SPLITS / MS_WAVE], l[MAX_SPLITS / MS_WAVE], top = -INFINITY, den = 0.f;
+#pragma unroll
+  for (int i = 0; i < MAX_SPLITS / MS_WAVE; ++i) {
+    const int s = lane + i * MS_WAVE;
+    m[i] = s < used ? part_ml[(slot0 + s) * 2] : -INFINITY;
+    l[i] = s < used ? part_ml[(slot0 + s) * 2 + 1] : 0.f;
+    top = fmaxf(top, m[i]);
+  }
+  top = wave_max(top);
+  if (top == -INFINITY) top = 0.f;
+#pragma unroll
+  for (int i = 0; i < MAX_SPLITS / MS_WAVE; ++i) {
+    m[i] = fast_exp2(m[i] - top);
+    den = fmaf(m[i], l[i], den);
+  }
+  den = wave_sum(den);
+  float acc[DL] = {};
+  for (int s = 0; s < used; ++s) {
+    const float w = __shfl(s < MS_WAVE ? m[0] : m[1], s & (MS_WAVE - 1), MS_WAVE);
+#pragma unroll
+    for (int e = 0; e < DL; ++e) acc[e] = fmaf(w, part_o[(slot0 + s) * D + min(lane + e * MS_WAVE, D - 1)], acc[e]);
+  }
+  const float inv = den != 0.f ? 1.0f / den : 0.f;
+#pragma unroll
+  for (int e = 0; e < DL; ++e)
+    if (lane + e * MS_WAVE < D) out[(size_t)n * out_stride + (size_t)h * D + lane + e * MS_WAVE] = __float2bfloat16(acc[e] * inv);
+}
+
+struct Call {
+  const bf16 *q, *k, *vt;
+  const int *table, *rows, *token_req, *q_start, *ctx;
+  const unsigned* tree;
+  bf16* out;
+  float *part_o, *part_ml;
+  size_t q_stride, out_stride;
+  int table_stride, words, n_requests, n_tokens, max_q_len, nh, nkv, page_size, n_splits;
+  float scale_log2e;
+  hipStream_t stream;
+};
+
+inline long long column_tiles(int n_requests, int n_tokens, int max_q_len, int rep, int cols) {
+  return std::min((long long)n_tokens * rep / cols + n_requests, ((long long)max_q_len * rep + cols - 1) / cols * n_requests);
+}
+
+template <int D, int WC, int KG, int NT>
+int launch(const Call& a) {
+  typedef Shape<D, WC, KG, NT> S;
+  static bool raised = false;   // once per instantiation: allow more LDS than the default 64 KB
+  if (!raised) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_attention_mfma_kernel<D, WC, KG, NT>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::LDS) != hipSuccess)
+      return MS_LAUNCH_FAILED;
+    raised = true;
+  }
+  const long long tiles = column_tiles(a.n_requests, a.n_tokens, a.max_q_len, a.nh / a.nkv, S::COLS);
+  if (tiles > 65535) return MS_UNSUPPORTED;
+  tree_attention_mfma_kernel<D, WC, KG, NT><<<dim3(a.nkv, (unsigned)tiles, a.n_splits), dim3(KG * WC * MS_WAVE), S::LDS, a.stream>>>(
+      a.q, a.q_stride, a.k, a.vt, a.table, a.table_stride, a.rows, a.q_start, a.ctx, a.tree, a.words, a.out, a.out_stride, a.part_o,
+      a.part_ml, a.nh, a.nkv, a.page_size, a.scale_log2e, a.n_requests, a.n_splits);
+  if (a.n_splits > 1) {
+    const long long items = (long long)a.n_tokens * a.nh;
+    tree_combine_kernel<D><<<dim3((unsigned)((items + COMBINE_WAVES - 1) / COMBINE_WAVES)), dim3(COMBINE_WAVES * MS_WAVE), 0, a.stream>>>(
+        a.part_o, a.part_ml, a.token_req, a.q_start, a.ctx, a.n_requests, a.out, a.out_stride, a.n_tokens, a.nh, S::KEYS, a.n_splits);
+  }
+  return ms_launch_status();
+}
+
+// Waves that own columns and their tiles of 16, by the columns of the largest tree.
+inline void shape_of(int max_cols, int& wc, int& nt) {
+  wc = max_cols <= 16 ? 1 : max_cols <= 32 ? 2 : 4;
+  nt = max_cols <= 64 ? 1 : 2;
+}
+
+}  // namespace
+
+// Blocks that share a request's keys out, for a step of these sizes (all bounds); 0: sizes this kernel does not take.
+// A block's chain should be as short as the chip has room for: about two blocks a CU, but no share smaller than one turn.
+extern "C" int ms_tree_attention_mfma_splits(int n_requests, int n_tokens, int max_q_len, int max_context_len, int num_heads,
+                                             int num_kv_heads, int head_dim, int page_size) {
+  if ((head_dim != 32 && head_dim != 64 && head_dim != 128) || page_size <= 0 || page_size % 16) return 0;
+  if (n_requests <= 0 || n_tokens <= 0 || max_q_len <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads) return 0;
+  const int rep = num_heads / num_kv_heads;
+  int wc, nt;
+  if ((long long)max_q_len * rep > 0x3fffffffLL) return 0;
+  shape_of(max_q_len * rep, wc, nt);
+  const long long blocks = column_tiles(n_requests, n_tokens, max_q_len, rep, wc * nt * 16) * num_kv_heads;
+  const int turn = (wc == 4 ? 64 : 32) * (head_dim == 128 ? 4 : 8) / wc;
+  const long long most = std::max(1, (max_context_len + turn - 1) / turn);
+  return (int)std::max(1LL, std::min<long long>(std::min<long long>(most, MAX_SPLITS), 2LL * ms_compute_units() / blocks));
+}
+
+// part_o: float [n_tokens, num_heads, n_splits, head_dim], part_ml: float [n_tokens, num_heads, n_splits, 2] (null with one).
+extern "C" int ms_tree_attention_mfma(const void* q, long long q_stride, const void* k_pages, const void* vt_pages,
+                                      const int* block_table, int table_stride, const int* table_rows, const int* token_req,
+                                      const int* q_start, const int* context_lens, const int* tree, int words, void* out,
+                                      long long out_stride, void* part_o, void* part_ml, int n_requests, int n_tokens,
+                                      int max_q_len, int num_heads, int num_kv_heads, int head_dim, int page_size, float scale,
+                                      int n_splits, hipStream_t stream) {
+  if (n_requests <= 0 || n_tokens <= 0 || max_q_len <= 0) return MS_OK;
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || table_stride <= 0 || words <= 0) return MS_BAD_ARG;
+  if (!(scale > 0.f)) return MS_UNSUPPORTED;   // maxima are taken of the raw scores
+  if (n_splits < 1 || n_splits > MAX_SPLITS || (n_splits > 1 && (part_o == nullptr || part_ml == nullptr))) return MS_BAD_ARG;
+  if (page_size <= 0 || page_size % 16 || num_kv_heads > 65535) return MS_UNSUPPORTED;
+  if (q_stride % 8 || out_stride % 4 || ((uintptr_t)q % 16) || ((uintptr_t)out % 8) || ((uintptr_t)part_o % 16)) return MS_UNSUPPORTED;
+  if (((uintptr_t)k_pages | (uintptr_t)vt_pages) % 16) return MS_UNSUPPORTED;
+  const int rep = num_heads / num_kv_heads;
+  if ((long long)max_q_len * rep > 0x3fffffffLL || (long long)n_tokens * num_heads > 0x3fffffffLL) return MS_UNSUPPORTED;
+  const Call a = {(const bf16*)q, (const bf16*)k_pages, (const bf16*)vt_pages, block_table, table_rows, token_req, q_start, context_lens,
+                  (const unsigned*)tree, (bf16*)out, (float*)part_o, (float*)part_ml, (size_t)q_stride, (size_t)out_stride, table_stride,
+                  words, n_requests, n_tokens, max_q_len, num_heads, num_kv_heads, page_size, n_splits, scale * 1.4426950408889634f, stream};
+  int wc, nt;
+  shape_of(max_q_len * rep, wc, nt);
+#define GO(D, G) do { if (wc == 1) return launch<D, 1, G, 1>(a); if (wc == 2) return launch<D, 2, G / 2, 1>(a); \
+                      if (nt == 1) return launch<D, 4, G / 4, 1>(a); return launch<D, 4, G / 4, 2>(a); } while (0)
+  if (head_dim == 32) GO(32, 8);
+  if (head_dim == 64) GO(64, 8);
+  if (head_dim == 128) GO(128, 4);
+#undef GO
+  return MS_UNSUPPORTED;
+}

@@ -122,6 +122,9 @@ _SIGNATURES = {
     "ms_tree_attention_generic": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                   _c_int, _c_ptr, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int,
                                   _c_ptr],
+    "ms_tree_attention_mfma_splits": [_c_int] * 8,
+    "ms_tree_attention_mfma": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr,
+                               _c_ll, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr],
     "ms_verify_drafts": [_c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr,
                          _c_ptr],
     "ms_keep_tokens_max": [],
@@ -1552,6 +1555,35 @@ def tree_attention_generic(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     return out
 
 
+def tree_attention_mfma(q: torch.Tensor, k_pages: torch.Tensor, vt_pages: torch.Tensor, block_table: torch.Tensor,
+                        token_req: torch.Tensor, q_start: torch.Tensor, context_lens: torch.Tensor, tree: torch.Tensor,
+                        out: torch.Tensor, num_heads: int, scale: float, max_q_len: int, max_context_len: int,
+                        table_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``tree_attention`` on the matrix cores: bfloat16, heads of 32, 64 or 128 entries, value pages of that size transposed,
+    pages of a multiple of 16 tokens, a positive scale.  ``max_q_len`` and ``max_context_len`` are upper bounds; tokens from
+    q_start[R] on belong to no request, a request may have no token."""
+    _check(k_pages, "k_pages", torch.bfloat16)
+    P, nkv, page_size, d = k_pages.shape
+    _check(vt_pages, "vt_pages", torch.bfloat16, (P, nkv, d, page_size))
+    q_stride = _tree_step(q, k_pages, block_table, q_start, context_lens, table_rows, out, num_heads, nkv, d, d, max_q_len)
+    N, R = q.shape[0], context_lens.numel()
+    words = _tree_words(tree, N, max_q_len)
+    _check(token_req, "token_req", torch.int32, (N,))
+    _here(q, k_pages, vt_pages, block_table, table_rows, token_req, q_start, context_lens, tree, out)
+    if N == 0 or R == 0:
+        return out
+    n_splits = _get("ms_tree_attention_mfma_splits")(R, N, max_q_len, max_context_len, num_heads, nkv, d, page_size)
+    part_o = part_ml = None
+    if n_splits > 1:
+        part_o = torch.empty((N, num_heads, n_splits, d), dtype=torch.float32, device=q.device)
+        part_ml = torch.empty((N, num_heads, n_splits, 2), dtype=torch.float32, device=q.device)
+    _call("ms_tree_attention_mfma", q.data_ptr(), q_stride, k_pages.data_ptr(), vt_pages.data_ptr(), block_table.data_ptr(),
+          block_table.shape[1], _ptr(table_rows), token_req.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(), tree.data_ptr(),
+          words, out.data_ptr(), num_heads * d, _ptr(part_o), _ptr(part_ml), R, N, max_q_len, num_heads, nkv, d, page_size, float(scale),
+          max(1, n_splits), _stream())
+    return out
+
+
 def _tree_step(q, k_pages, block_table, q_start, context_lens, table_rows, out, num_heads, nkv, d, dv, max_q_len) -> int:
     """Checks what the kernels of ``tree_attention`` have in common; the stride of q's rows."""
     stride = _rows2d(q, "q", k_pages.dtype)
@@ -1582,6 +1614,11 @@ def tree_attention(q: torch.Tensor, kv, ctx, tree: torch.Tensor, out: torch.Tens
     The step's keys and values lie in the cache in the order of the tokens (``slot_mapping``), encoded with whatever
     positions the tree gives them; ``keep_tokens`` moves together what is accepted."""
     d, page_size = kv.k_pages.shape[3], kv.k_pages.shape[2]
+    if (q.dtype == torch.bfloat16 and kv.v_transposed and kv.v_pages.shape[2] == d and attention_mfma_supported(d, page_size) and scale > 0
+            and kv.k_pages.data_ptr() % 16 == 0 and kv.v_pages.data_ptr() % 16 == 0 and q.data_ptr() % 16 == 0
+            and out.data_ptr() % 8 == 0 and (q.shape[0] == 1 or q.stride(0) % 8 == 0)):
+        return tree_attention_mfma(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.q_start, ctx.context_lens, tree, out,
+                                   num_heads, scale, max(1, ctx.max_q_len), max(1, ctx.max_context_len), kv.table_rows)
     return tree_attention_generic(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.q_start, ctx.context_lens, tree,
                                   out, num_heads, scale, max(1, ctx.max_q_len), kv.v_transposed, kv.table_rows, ctx.n_live_tokens)
 
