@@ -252,15 +252,15 @@ int ms_tree_attention_generic(const void* q, long long q_stride, const void* k_p
                               int page_size, float scale, int v_transposed, int dtype, hipStream_t stream);
 
 // The same on the matrix cores: bfloat16, head sizes 32, 64 and 128, values of that size in transposed pages, pages of a multiple
-// of 16.  The keys of a request go to n_splits blocks (ms_tree_attention_mfma_splits; 0: not its sizes), whose results part_o
+// of 16.  The keys of a request go to n_splits blocks (ms_tree_attention_mfma_plan: kind * 65536 + share / 64; -1: not its sizes), whose results part_o
 // float [n_tokens, num_heads, n_splits, head_dim] and part_ml float [n_tokens, num_heads, n_splits, 2] a second kernel adds up.
-int ms_tree_attention_mfma_splits(int n_requests, int n_tokens, int max_q_len, int max_context_len, int num_heads,
-                                  int num_kv_heads, int head_dim, int page_size);
+int ms_tree_attention_mfma_plan(int n_requests, int n_tokens, int max_q_len, int max_context_len, int num_heads,
+                                int num_kv_heads, int head_dim, int page_size);
 int ms_tree_attention_mfma(const void* q, long long q_stride, const void* k_pages, const void* vt_pages, const int* block_table,
                            int table_stride, const int* table_rows, const int* token_req, const int* q_start,
                            const int* context_lens, const int* tree, int words, void* out, long long out_stride, void* part_o,
                            void* part_ml, int n_requests, int n_tokens, int max_q_len, int num_heads, int num_kv_heads,
-                           int head_dim, int page_size, float scale, int n_splits, hipStream_t stream);
+                           int head_dim, int page_size, float scale, int kind, int share, int n_splits, hipStream_t stream);
 
 // p, q [n_tokens, vocab] (q may be null), tokens / parents / uniforms [n_tokens], q_start [n_requests + 1] -> nodes
 // [n_requests, depth] (the accepted path, -1 behind it), counts [n_requests], out [n_requests] (the token drawn behind it).

@@ -41,11 +41,6 @@ __device__ __forceinline__ float column_max(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// Which of the n_splits shares of a request's tiles of keys a block has; the shares are even, the last ones may be empty.
-__device__ __forceinline__ int tiles_a_split(int context, int keys, int n_splits) {
-  return ((context + keys - 1) / keys + n_splits - 1) / n_splits;
-}
-
 template <int D, int WC, int KG, int NT>
 struct Shape {
   static constexpr int COLS = WC * NT * 16, KEYS = WC == 4 ? 64 : 32, CHUNKS = KEYS / 16;
@@ -55,16 +50,17 @@ struct Shape {
 };
 
 template <int D, int WC, int KG, int NT>
-__global__ void __launch_bounds__(KG * WC * MS_WAVE, D == 128 ? 2 : 4)
+__global__ void __launch_bounds__(KG * WC * MS_WAVE, D == 128 || NT == 2 ? 2 : 4)
 tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf16* __restrict__ k_pages,
                            const bf16* __restrict__ vt_pages, const int* __restrict__ block_table, int table_stride,
                            const int* __restrict__ table_rows, const int* __restrict__ q_start,
                            const int* __restrict__ context_lens, const unsigned* __restrict__ tree, int words,
                            bf16* __restrict__ out, size_t out_stride, float* __restrict__ part_o, float* __restrict__ part_ml,
-                           int nh, int nkv, int page_size, float scale_log2e, int n_requests, int n_splits) {
+                           int nh, int nkv, int page_size, float scale_log2e, int n_requests, int n_splits, int per) {      // n_requests 0: a tile to a request
   typedef Shape<D, WC, KG, NT> S;
   constexpr int COLS = S::COLS, KEYS = S::KEYS, CHUNKS = S::CHUNKS, CHUNK = S::CHUNK, STAGE = S::STAGE;
   constexpr int CT = D / 16, PIECES = D / 8, LOADS = CHUNK * 2 / 1024, MINE = CHUNKS / WC;      // chunks a wave brings
+  constexpr int UNITS = NT == 1 ? KEYS / 32 : 1;      // of 32 keys that go through the stages of a tile together
   extern __shared__ __align__(16) unsigned char lds_raw[];
   bf16* lds = reinterpret_cast<bf16*>(lds_raw);       // [KG][2 tiles][STAGE]
   const int lane = threadIdx.x & (MS_WAVE - 1);
@@ -74,13 +70,16 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
   const int g = blockIdx.x, rep = nh / nkv, split = blockIdx.z;
 
   int r, tile, n_tiles;
-  find_tile(q_start, n_requests, rep, COLS, blockIdx.y, lane, r, tile, n_tiles);
-  if (r < 0) return;
+  if (n_requests == 0) {
+    r = blockIdx.y; tile = 0;
+  } else {
+    find_tile(q_start, n_requests, rep, COLS, blockIdx.y, lane, r, tile, n_tiles);
+    if (r < 0) return;
+  }
   const int* table = block_table + (size_t)(table_rows ? table_rows[r] : r) * table_stride;
   const int q0 = q_start[r], qlen = q_start[r + 1] - q0, context = context_lens[r], before = context - qlen, ncols = qlen * rep;
-  const int per = tiles_a_split(context, KEYS, n_splits);
   const int t_begin = split * per, t_end = min((context + KEYS - 1) / KEYS, t_begin + per);
-  if (t_begin >= t_end) return;
+  if (t_begin >= t_end || qlen <= 0) return;
   const int c0 = (tile * WC + wave) * NT * 16;
   const bool works = c0 < ncols;       // without columns a wave still brings its chunks
 
@@ -125,16 +124,15 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
 
   // ---- this lane's columns
   bool idle[NT];
-  const unsigned* mask[NT];
   unsigned first_words[NT][2];         // (most trees have no more)
   bf16x8 qv[NT][D / 32];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int c = c0 + t * 16 + col16, cc = min(c, ncols - 1), tok = q0 + cc / rep;
     idle[t] = c >= ncols;
-    mask[t] = tree + (size_t)tok * words;
-    first_words[t][0] = mask[t][0];
-    first_words[t][1] = words > 1 ? mask[t][1] : 0u;
+    const unsigned* mask = tree + (size_t)tok * words;
+    first_words[t][0] = mask[0];
+    first_words[t][1] = words > 1 ? mask[1] : 0u;
     const bf16* qp = q + (size_t)tok * q_stride + (size_t)(g * rep + cc % rep) * D + kq * 8;
 #pragma unroll
     for (int s = 0; s < D / 32; ++s) qv[t][s] = *reinterpret_cast<const bf16x8*>(qp + s * 32);
@@ -145,7 +143,7 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
     if (idle[t]) return 0u;
     if (rel <= -8) return 0xffu;
     const int at = max(rel, 0), w = at >> 5;
-    auto word = [&](int i) -> unsigned { return i == 0 ? first_words[t][0] : i == 1 ? first_words[t][1] : i < words ? mask[t][i] : 0u; };
+    auto word = [&](int i) -> unsigned { return i == 0 ? first_words[t][0] : i == 1 ? first_words[t][1] : i < words ? tree[(size_t)(q0 + (c0 + t * 16 + col16) / rep) * words + i] : 0u; };
     unsigned bits = (unsigned)((((unsigned long long)word(w + 1) << 32) | word(w)) >> (at & 31)) & 0xffu;
     if (rel < 0) bits = ((bits << -rel) | ((1u << -rel) - 1u)) & 0xffu;
     const int left = qlen - rel;
@@ -188,115 +186,140 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
     }
     if (!works || t >= t_end) continue;      // the same for the whole wave
 #pragma unroll
-    for (int unit = 0; unit < KEYS / 32; ++unit) {
-      const int base = t * KEYS + unit * 32;
-      if (base >= context) break;
-      const bf16* st = lds + (kg * 2 + stage) * STAGE + unit * 2 * CHUNK;
+    for (int unit = 0; unit < KEYS / 32; unit += UNITS) {
+    const int base = t * KEYS + unit * 32;
+    const bf16* st = lds + (kg * 2 + stage) * STAGE + unit * 2 * CHUNK;
 
-      // scores: s[u][t] holds keys base + kq*8 + u*4 + (0..3) of column t*16 + col16
-      f32x4 s[2][NT];
+    // scores: s[n][u][t] holds keys base + n*32 + kq*8 + u*4 + (0..3) of column t*16 + col16.  The units of a tile go through
+    // every stage together: a wave's products wait for each other (0.9 us a unit of 32 keys where a CU has one block, 0.45 of
+    // them products), and those of another unit can run meanwhile.
+    f32x4 s[UNITS][2][NT];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+    for (int n = 0; n < UNITS; ++n)
 #pragma unroll
-        for (int t2 = 0; t2 < NT; ++t2) s[u][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int ks = 0; ks < D / 32; ++ks) {
-          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(st + k_row[u] + (((ks * 4 + kq) ^ k_perm[u]) & (PIECES - 1)) * 8);
+        for (int t2 = 0; t2 < NT; ++t2) s[n][u][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int t2 = 0; t2 < NT; ++t2) s[u][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qv[t2][ks], s[u][t2], 0, 0, 0);
+    for (int ks = 0; ks < D / 32; ++ks)
+#pragma unroll
+      for (int n = 0; n < UNITS; ++n)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(st + n * 2 * CHUNK + k_row[u] + (((ks * 4 + kq) ^ k_perm[u]) & (PIECES - 1)) * 8);
+#pragma unroll
+          for (int t2 = 0; t2 < NT; ++t2) s[n][u][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qv[t2][ks], s[n][u][t2], 0, 0, 0);
         }
-      }
-      const bool masked = base + 31 >= before;     // reaches into the step's own entries, or behind them
-      unsigned sees[NT];
-      if (masked) {
+    const bool masked = base + UNITS * 32 > before;     // reaches into the step's own entries, or behind them
+    unsigned sees[UNITS][NT];
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < UNITS; ++n)
 #pragma unroll
         for (int t2 = 0; t2 < NT; ++t2) {
-          sees[t2] = visible(t2, base);
+          sees[n][t2] = visible(t2, base + n * 32);
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (!((sees[t2] >> (u * 4 + i)) & 1u)) s[u][t2][i] = -INFINITY;
+              if (!((sees[n][t2] >> (u * 4 + i)) & 1u)) s[n][u][t2][i] = -INFINITY;
         }
-      }
-      // m is the reference of the exponents: it follows the maximum when that has run ahead by REF_SLACK
-      float bmax[NT];
-      bool ahead = false;
+    }
+    // m is the reference of the exponents: it follows the maximum when that has run ahead by REF_SLACK
+    float bmax[NT];
+    bool ahead = false;
 #pragma unroll
-      for (int t2 = 0; t2 < NT; ++t2) {
-        float bm = -INFINITY;
+    for (int t2 = 0; t2 < NT; ++t2) {
+      float bm = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < UNITS; ++n)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) bm = fmaxf(bm, s[u][t2][i]);
-        bmax[t2] = bm;
-        ahead |= bm * scale_log2e > m[t2] + REF_SLACK;
-      }
-      if (__builtin_amdgcn_ballot_w64(ahead) != 0) {
+          for (int i = 0; i < 4; ++i) bm = fmaxf(bm, s[n][u][t2][i]);
+      bmax[t2] = bm;
+      ahead |= bm * scale_log2e > m[t2] + REF_SLACK;
+    }
+    if (__builtin_amdgcn_ballot_w64(ahead) != 0) {
 #pragma unroll
-        for (int t2 = 0; t2 < NT; ++t2) {
-          const float bm = column_max(bmax[t2]) * scale_log2e;
-          const bool step = bm > m[t2] + REF_SLACK;
-          const float corr = step ? fast_exp2(m[t2] - bm) : 1.0f;      // m = -inf: 0
-          if (step) m[t2] = bm;
-          lsum[t2] *= corr;
+      for (int t2 = 0; t2 < NT; ++t2) {
+        const float bm = column_max(bmax[t2]) * scale_log2e;
+        const bool step = bm > m[t2] + REF_SLACK;
+        const float corr = step ? fast_exp2(m[t2] - bm) : 1.0f;      // m = -inf: 0
+        if (step) m[t2] = bm;
+        lsum[t2] *= corr;
 #pragma unroll
-          for (int c = 0; c < CT; ++c) o[c][t2] *= corr;
-        }
+        for (int c = 0; c < CT; ++c) o[c][t2] *= corr;
       }
-      bf16x8 p[NT];
+    }
+    bf16x8 p[UNITS][NT];
+#pragma unroll
+    for (int n = 0; n < UNITS; ++n)
 #pragma unroll
       for (int t2 = 0; t2 < NT; ++t2) {
         const float ref = m[t2] == -INFINITY ? 0.f : m[t2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[t2][u * 4 + i] = (__bf16)fast_exp2(fmaf(s[u][t2][i], scale_log2e, -ref));
-        lsum[t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[t2], lsum[t2], 0, 0, 0);
+          for (int i = 0; i < 4; ++i) p[n][t2][u * 4 + i] = (__bf16)fast_exp2(fmaf(s[n][u][t2][i], scale_log2e, -ref));
+        lsum[t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[n][t2], lsum[t2], 0, 0, 0);
       }
-      bool spoiled = false;      // some value of the step's own entries that is not finite
+    if (!masked) {
+#pragma unroll
+      for (int n = 0; n < UNITS; ++n)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          const bf16x8 v = *reinterpret_cast<const bf16x8*>(st + n * 2 * CHUNK + v_row + c * 256);
+#pragma unroll
+          for (int t2 = 0; t2 < NT; ++t2) o[c][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[n][t2], o[c][t2], 0, 0, 0);
+        }
+      continue;
+    }
+    // Values behind the context may be anything a reused page still holds: zeros.  Those of the step's entries that are not
+    // finite would reach columns that do not see them: zeros here, and added below for those that do.
+    bool spoiled = false;
+#pragma unroll
+    for (int n = 0; n < UNITS; ++n)
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        bf16x8 v = *reinterpret_cast<const bf16x8*>(st + v_row + c * 256);
-        if (masked) {
-          // Values behind the context may be anything a reused page still holds: zeros.  Those of the step's entries that are
-          // not finite would reach columns that do not see them: zeros here, and added below for those that do.
-          u16x8 raw = __builtin_bit_cast(u16x8, v);
+        u16x8 raw = *reinterpret_cast<const u16x8*>(st + n * 2 * CHUNK + v_row + c * 256);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int key = base + kq * 8 + i;
-            const bool wild = key >= before && (raw[i] & 0x7f80) == 0x7f80;
-            spoiled |= wild && key < context;
-            if (wild || key >= context) raw[i] = 0;
-          }
-          v = __builtin_bit_cast(bf16x8, raw);
+        for (int i = 0; i < 8; ++i) {
+          const int key = base + n * 32 + kq * 8 + i;
+          const bool wild = (key >= before) & ((raw[i] & 0x7f80) == 0x7f80), gone = key >= context;
+          spoiled |= wild & !gone;
+          raw[i] = wild | gone ? (unsigned short)0 : raw[i];
         }
+        const bf16x8 v = __builtin_bit_cast(bf16x8, raw);
 #pragma unroll
-        for (int t2 = 0; t2 < NT; ++t2) o[c][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t2], o[c][t2], 0, 0, 0);
+        for (int t2 = 0; t2 < NT; ++t2) o[c][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[n][t2], o[c][t2], 0, 0, 0);
       }
-      if (masked && __builtin_amdgcn_ballot_w64(spoiled) != 0) {
+    if (__builtin_amdgcn_ballot_w64(spoiled) != 0) {
+#pragma unroll
+      for (int n = 0; n < UNITS; ++n)
         for (int k = 0; k < 32; ++k) {
-          if (base + k < before || base + k >= context) continue;
+          const int key = base + n * 32 + k;
+          if (key < before || key >= context) continue;
           const int owner = (k >> 3) * 16 + col16;
 #pragma unroll
           for (int t2 = 0; t2 < NT; ++t2) {
             float mine = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mine = (k & 7) == i ? (float)p[t2][i] : mine;
+            for (int i = 0; i < 8; ++i) mine = (k & 7) == i ? (float)p[n][t2][i] : mine;
             const float w = __shfl(mine, owner, MS_WAVE);
-            const bool see = (__shfl(sees[t2], owner, MS_WAVE) >> (k & 7)) & 1u;
+            const bool see = (__shfl(sees[n][t2], owner, MS_WAVE) >> (k & 7)) & 1u;
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int dim = c * 16 + kq * 4 + i;
                 const unsigned short raw = __builtin_bit_cast(unsigned short,
-                    st[CHUNKS * CHUNK + (k >> 4) * CHUNK + dim * 16 + ((((k >> 3) ^ (dim >> 3)) & 1) * 8) + (k & 7)]);
+                    st[CHUNKS * CHUNK + (n * 2 + (k >> 4)) * CHUNK + dim * 16 + ((((k >> 3) ^ (dim >> 3)) & 1) * 8) + (k & 7)]);
                 if (see && (raw & 0x7f80u) == 0x7f80u) o[c][t2][i] += w * __uint_as_float((unsigned)raw << 16);
               }
           }
         }
-      }
+    }
     }
   }
 
@@ -375,14 +398,14 @@ template <int D>
 __global__ void __launch_bounds__(COMBINE_WAVES * MS_WAVE)
 tree_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ token_req,
                     const int* __restrict__ q_start, const int* __restrict__ context_lens, int n_requests, bf16* __restrict__ out,
-                    size_t out_stride, int n_tokens, int nh, int keys, int n_splits) {
+                    size_t out_stride, int n_tokens, int nh, int share, int n_splits) {
   constexpr int DL = (D + MS_WAVE - 1) / MS_WAVE;
   const int lane = threadIdx.x & (MS_WAVE - 1);
   const long long item = (long long)blockIdx.x * COMBINE_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / MS_WAVE);
   const int n = (int)(item / nh), h = (int)(item - (long long)n * nh);
   if (n >= n_tokens || n >= q_start[n_requests]) return;      // (a token that pads a captured batch)
   const int context = context_lens[token_req[n]];
-  const int per = tiles_a_split(context, keys, n_splits), used = ((context + keys - 1) / keys + per - 1) / per;
+  const int used = min((context + share - 1) / share, n_splits);
   const size_t slot0 = (size_t)item * n_splits;
   float m[MAX_SPLITS / MS_WAVE], l[MAX_SPLITS / MS_WAVE], top = -INFINITY, den = 0.f;
 #pragma unroll
@@ -419,7 +442,7 @@ struct Call {
   bf16* out;
   float *part_o, *part_ml;
   size_t q_stride, out_stride;
-  int table_stride, words, n_requests, n_tokens, max_q_len, nh, nkv, page_size, n_splits;
+  int table_stride, words, n_requests, n_tokens, max_q_len, nh, nkv, page_size, n_splits, share;
   float scale_log2e;
   hipStream_t stream;
 };
@@ -438,41 +461,44 @@ int launch(const Call& a) {
       return MS_LAUNCH_FAILED;
     raised = true;
   }
-  const long long tiles = column_tiles(a.n_requests, a.n_tokens, a.max_q_len, a.nh / a.nkv, S::COLS);
+  const int rep = a.nh / a.nkv;
+  const bool one = (long long)a.max_q_len * rep <= S::COLS;
+  const long long tiles = one ? a.n_requests : column_tiles(a.n_requests, a.n_tokens, a.max_q_len, rep, S::COLS);
   if (tiles > 65535) return MS_UNSUPPORTED;
   tree_attention_mfma_kernel<D, WC, KG, NT><<<dim3(a.nkv, (unsigned)tiles, a.n_splits), dim3(KG * WC * MS_WAVE), S::LDS, a.stream>>>(
       a.q, a.q_stride, a.k, a.vt, a.table, a.table_stride, a.rows, a.q_start, a.ctx, a.tree, a.words, a.out, a.out_stride, a.part_o,
-      a.part_ml, a.nh, a.nkv, a.page_size, a.scale_log2e, a.n_requests, a.n_splits);
+      a.part_ml, a.nh, a.nkv, a.page_size, a.scale_log2e, one ? 0 : a.n_requests, a.n_splits, a.share / S::KEYS);
   if (a.n_splits > 1) {
     const long long items = (long long)a.n_tokens * a.nh;
     tree_combine_kernel<D><<<dim3((unsigned)((items + COMBINE_WAVES - 1) / COMBINE_WAVES)), dim3(COMBINE_WAVES * MS_WAVE), 0, a.stream>>>(
-        a.part_o, a.part_ml, a.token_req, a.q_start, a.ctx, a.n_requests, a.out, a.out_stride, a.n_tokens, a.nh, S::KEYS, a.n_splits);
+        a.part_o, a.part_ml, a.token_req, a.q_start, a.ctx, a.n_requests, a.out, a.out_stride, a.n_tokens, a.nh, a.share, a.n_splits);
   }
   return ms_launch_status();
 }
 
-// Waves that own columns and their tiles of 16, by the columns of the largest tree.
-inline void shape_of(int max_cols, int& wc, int& nt) {
-  wc = max_cols <= 16 ? 1 : max_cols <= 32 ? 2 : 4;
-  nt = max_cols <= 64 ? 1 : 2;
-}
+// Kinds of block: WC waves over columns, KG groups over keys (twice as many below 128 dims), NT tiles of 16 columns a wave.
+struct Kind { int wc, kg, nt; };
+constexpr Kind KINDS[] = {{1, 4, 1}, {2, 2, 1}, {4, 1, 1}, {4, 1, 2}, {4, 2, 1}, {4, 2, 2}};
+constexpr int N_KINDS = sizeof(KINDS) / sizeof(KINDS[0]);
 
 }  // namespace
 
-// Blocks that share a request's keys out, for a step of these sizes (all bounds); 0: sizes this kernel does not take.
-// A block's chain should be as short as the chip has room for: about two blocks a CU, but no share smaller than one turn.
-extern "C" int ms_tree_attention_mfma_splits(int n_requests, int n_tokens, int max_q_len, int max_context_len, int num_heads,
-                                             int num_kv_heads, int head_dim, int page_size) {
-  if ((head_dim != 32 && head_dim != 64 && head_dim != 128) || page_size <= 0 || page_size % 16) return 0;
-  if (n_requests <= 0 || n_tokens <= 0 || max_q_len <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads) return 0;
+// kind * 65536 + how many times 64 keys a block takes, for a step of these sizes (all bounds); -1: sizes this kernel does
+// not take.
+extern "C" int ms_tree_attention_mfma_plan(int n_requests, int n_tokens, int max_q_len, int max_context_len, int num_heads,
+                                           int num_kv_heads, int head_dim, int page_size) {
+  if ((head_dim != 32 && head_dim != 64 && head_dim != 128) || page_size <= 0 || page_size % 16) return -1;
+  if (n_requests <= 0 || n_tokens <= 0 || max_q_len <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads) return -1;
   const int rep = num_heads / num_kv_heads;
-  int wc, nt;
-  if ((long long)max_q_len * rep > 0x3fffffffLL) return 0;
-  shape_of(max_q_len * rep, wc, nt);
-  const long long blocks = column_tiles(n_requests, n_tokens, max_q_len, rep, wc * nt * 16) * num_kv_heads;
-  const int turn = (wc == 4 ? 64 : 32) * (head_dim == 128 ? 4 : 8) / wc;
+  if ((long long)max_q_len * rep > 0x3fffffffLL) return -1;
+  const int cols = max_q_len * rep;
+  const int kind = cols <= 16 ? 0 : cols <= 32 ? 1 : cols <= 64 ? 2 : 3;
+  const Kind k = KINDS[kind];
+  const long long blocks = column_tiles(n_requests, n_tokens, max_q_len, rep, k.wc * k.nt * 16) * num_kv_heads;
+  const int turn = (k.wc == 4 ? 64 : 32) * k.kg * (head_dim == 128 ? 1 : 2);
   const long long most = std::max(1, (max_context_len + turn - 1) / turn);
-  return (int)std::max(1LL, std::min<long long>(std::min<long long>(most, MAX_SPLITS), 2LL * ms_compute_units() / blocks));
+  const int splits = (int)std::max(1LL, std::min<long long>(std::min<long long>(most, MAX_SPLITS), 2LL * ms_compute_units() / blocks));
+  return kind * 65536 + ((max_context_len + splits - 1) / splits + 63) / 64;
 }
 
 // part_o: float [n_tokens, num_heads, n_splits, head_dim], part_ml: float [n_tokens, num_heads, n_splits, 2] (null with one).
@@ -481,10 +507,11 @@ extern "C" int ms_tree_attention_mfma(const void* q, long long q_stride, const v
                                       const int* q_start, const int* context_lens, const int* tree, int words, void* out,
                                       long long out_stride, void* part_o, void* part_ml, int n_requests, int n_tokens,
                                       int max_q_len, int num_heads, int num_kv_heads, int head_dim, int page_size, float scale,
-                                      int n_splits, hipStream_t stream) {
+                                      int kind, int share, int n_splits, hipStream_t stream) {
   if (n_requests <= 0 || n_tokens <= 0 || max_q_len <= 0) return MS_OK;
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || table_stride <= 0 || words <= 0) return MS_BAD_ARG;
   if (!(scale > 0.f)) return MS_UNSUPPORTED;   // maxima are taken of the raw scores
+  if (share <= 0 || share % 64) return MS_BAD_ARG;
   if (n_splits < 1 || n_splits > MAX_SPLITS || (n_splits > 1 && (part_o == nullptr || part_ml == nullptr))) return MS_BAD_ARG;
   if (page_size <= 0 || page_size % 16 || num_kv_heads > 65535) return MS_UNSUPPORTED;
   if (q_stride % 8 || out_stride % 4 || ((uintptr_t)q % 16) || ((uintptr_t)out % 8) || ((uintptr_t)part_o % 16)) return MS_UNSUPPORTED;
@@ -493,14 +520,13 @@ extern "C" int ms_tree_attention_mfma(const void* q, long long q_stride, const v
   if ((long long)max_q_len * rep > 0x3fffffffLL || (long long)n_tokens * num_heads > 0x3fffffffLL) return MS_UNSUPPORTED;
   const Call a = {(const bf16*)q, (const bf16*)k_pages, (const bf16*)vt_pages, block_table, table_rows, token_req, q_start, context_lens,
                   (const unsigned*)tree, (bf16*)out, (float*)part_o, (float*)part_ml, (size_t)q_stride, (size_t)out_stride, table_stride,
-                  words, n_requests, n_tokens, max_q_len, num_heads, num_kv_heads, page_size, n_splits, scale * 1.4426950408889634f, stream};
-  int wc, nt;
-  shape_of(max_q_len * rep, wc, nt);
-#define GO(D, G) do { if (wc == 1) return launch<D, 1, G, 1>(a); if (wc == 2) return launch<D, 2, G / 2, 1>(a); \
-                      if (nt == 1) return launch<D, 4, G / 4, 1>(a); return launch<D, 4, G / 4, 2>(a); } while (0)
-  if (head_dim == 32) GO(32, 8);
-  if (head_dim == 64) GO(64, 8);
-  if (head_dim == 128) GO(128, 4);
+                  words, n_requests, n_tokens, max_q_len, num_heads, num_kv_heads, page_size, n_splits, share, scale * 1.4426950408889634f, stream};
+#define GO(D, F) switch (kind) { case 0: return launch<D, 1, 4 * F, 1>(a); case 1: return launch<D, 2, 2 * F, 1>(a); \
+                                 case 2: return launch<D, 4, F, 1>(a); case 3: return launch<D, 4, 1, 2>(a); \
+                                 case 4: return launch<D, 4, 2 * F, 1>(a); case 5: return launch<D, 4, 2, 2>(a); }
+  if (head_dim == 32) GO(32, 2);
+  if (head_dim == 64) GO(64, 2);
+  if (head_dim == 128) GO(128, 1);
 #undef GO
   return MS_UNSUPPORTED;
 }

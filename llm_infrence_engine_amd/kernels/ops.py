@@ -122,9 +122,9 @@ _SIGNATURES = {
     "ms_tree_attention_generic": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                   _c_int, _c_ptr, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int,
                                   _c_ptr],
-    "ms_tree_attention_mfma_splits": [_c_int] * 8,
+    "ms_tree_attention_mfma_plan": [_c_int] * 8,
     "ms_tree_attention_mfma": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr,
-                               _c_ll, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr],
+                               _c_ll, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int, _c_ptr],
     "ms_verify_drafts": [_c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr,
                          _c_ptr],
     "ms_keep_tokens_max": [],
@@ -1572,15 +1572,17 @@ def tree_attention_mfma(q: torch.Tensor, k_pages: torch.Tensor, vt_pages: torch.
     _here(q, k_pages, vt_pages, block_table, table_rows, token_req, q_start, context_lens, tree, out)
     if N == 0 or R == 0:
         return out
-    n_splits = _get("ms_tree_attention_mfma_splits")(R, N, max_q_len, max_context_len, num_heads, nkv, d, page_size)
+    plan = _get("ms_tree_attention_mfma_plan")(R, N, max_q_len, max_context_len, num_heads, nkv, d, page_size)
+    kind, share = (plan >> 16, (plan & 0xFFFF) * 64) if plan >= 0 else (0, 64)
+    n_splits = -(-max_context_len // share)
     part_o = part_ml = None
     if n_splits > 1:
-        part_o = torch.empty((N, num_heads, n_splits, d), dtype=torch.float32, device=q.device)
-        part_ml = torch.empty((N, num_heads, n_splits, 2), dtype=torch.float32, device=q.device)
+        parts = torch.empty(N * num_heads * n_splits * (d + 2), dtype=torch.float32, device=q.device)
+        part_o, part_ml = parts.data_ptr(), parts.data_ptr() + 4 * N * num_heads * n_splits * d
     _call("ms_tree_attention_mfma", q.data_ptr(), q_stride, k_pages.data_ptr(), vt_pages.data_ptr(), block_table.data_ptr(),
           block_table.shape[1], _ptr(table_rows), token_req.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(), tree.data_ptr(),
-          words, out.data_ptr(), num_heads * d, _ptr(part_o), _ptr(part_ml), R, N, max_q_len, num_heads, nkv, d, page_size, float(scale),
-          max(1, n_splits), _stream())
+          words, out.data_ptr(), num_heads * d, part_o, part_ml, R, N, max_q_len, num_heads, nkv, d, page_size, float(scale),
+          kind, share, n_splits, _stream())
     return out
 
 
