@@ -56,7 +56,7 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
                            const int* __restrict__ table_rows, const int* __restrict__ q_start,
                            const int* __restrict__ context_lens, const unsigned* __restrict__ tree, int words,
                            bf16* __restrict__ out, size_t out_stride, float* __restrict__ part_o, float* __restrict__ part_ml,
-                           int nh, int nkv, int page_size, float scale_log2e, int n_requests, int n_splits, int per) {      // n_requests 0: a tile to a request
+                           int nh, int nkv, int page_size, int page_shift, float scale_log2e, int n_requests, int n_splits, int per) {      // n_requests 0: a tile to a request
   typedef Shape<D, WC, KG, NT> S;
   constexpr int COLS = S::COLS, KEYS = S::KEYS, CHUNKS = S::CHUNKS, CHUNK = S::CHUNK, STAGE = S::STAGE;
   constexpr int CT = D / 16, PIECES = D / 8, LOADS = CHUNK * 2 / 1024, MINE = CHUNKS / WC;      // chunks a wave brings
@@ -84,32 +84,62 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
   const bool works = c0 < ncols;       // without columns a wave still brings its chunks
 
   // ---- bringing a tile: the wave's chunks of keys and of values
-  int k_src[MINE][LOADS], v_src[LOADS];                        // what a lane asks for, from the chunk's first value in the page
+  unsigned k_src[MINE][LOADS], v_src[LOADS];                   // what a lane asks for, in bytes from the chunk's first value
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) {
     const int at = j * 512 + lane * 8, key = at / D, piece = (at % D) / 8;
 #pragma unroll
-    for (int b = 0; b < MINE; ++b) k_src[b][j] = key * D + (piece ^ permute<D>(((wave * MINE + b) & 1) * 16 + key)) * 8;
+    for (int b = 0; b < MINE; ++b) k_src[b][j] = (key * D + (piece ^ permute<D>(((wave * MINE + b) & 1) * 16 + key)) * 8) * 2;
     const int dim = at / 16, half = (at >> 3) & 1;
-    v_src[j] = dim * page_size + (half ^ ((dim >> 3) & 1)) * 8;
+    v_src[j] = (dim * page_size + (half ^ ((dim >> 3) & 1)) * 8) * 2;
   }
+  const size_t page_bytes = (size_t)nkv * page_size * D * 2, head_bytes = (size_t)g * page_size * D * 2;
+  const char *k_head = (const char*)k_pages + head_bytes, *v_head = (const char*)vt_pages + head_bytes;
   auto page_of = [&](int t, int b) {        // the page of one of the wave's chunks of tile t; past the context: the null page
     const int key = t * KEYS + (wave * MINE + b) * 16;
-    return key < context ? __builtin_amdgcn_readfirstlane(table[key / page_size]) : 0;
+    return key < context ? __builtin_amdgcn_readfirstlane(table[page_shift >= 0 ? key >> page_shift : key / page_size]) : 0;
   };
   auto bring = [&](int t, const int* pages, int stage) {
 #pragma unroll
     for (int b = 0; b < MINE; ++b) {
-      const int off = (t * KEYS + (wave * MINE + b) * 16) % page_size;
-      const size_t head = ((size_t)pages[b] * nkv + g) * page_size * D;
-      const bf16* kp = k_pages + head + (size_t)off * D;
-      const bf16* vp = vt_pages + head + off;
+      const int key = t * KEYS + (wave * MINE + b) * 16, off = page_shift >= 0 ? key & (page_size - 1) : key % page_size;
+      const size_t page = pages[b] * page_bytes;
+      const char *kp = k_head + page + off * (D * 2), *vp = v_head + page + off * 2;
       bf16* to = lds + (kg * 2 + stage) * STAGE + (wave * MINE + b) * CHUNK;
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) __builtin_amdgcn_global_load_lds((global_void*)(kp + k_src[b][j]), (lds_void*)(to + j * 512), 16, 0, 0);
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) __builtin_amdgcn_global_load_lds((global_void*)(vp + v_src[j]), (lds_void*)(to + CHUNKS * CHUNK + j * 512), 16, 0, 0);
     }
+  };
+  // Values behind the context may be anything a reused page still holds, and of the step's own entries those that are not
+  // finite would reach columns that do not see them (a NaN times a weight of zero): the wave that brought them makes them
+  // zeros, and says of the latter that they have to be added for the columns that do (`spoiled`: the tile, counted from 1).
+  __shared__ int spoiled[KG][2];
+  const bool some_masked = t_end * KEYS > before;
+  if (some_masked) {
+    if (threadIdx.x < 2 * KG) spoiled[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+    __syncthreads();
+  }
+  auto tidy = [&](int t, int stage) {
+    bool wild = false;
+#pragma unroll
+    for (int b = 0; b < MINE; ++b)
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int at = j * 512 + lane * 8, dim = at / 16, half = ((at >> 3) ^ (dim >> 3)) & 1;
+        u16x8* place = reinterpret_cast<u16x8*>(lds + (kg * 2 + stage) * STAGE + CHUNKS * CHUNK + (wave * MINE + b) * CHUNK + at);
+        u16x8 raw = *place;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = t * KEYS + (wave * MINE + b) * 16 + half * 8 + i;
+          const bool gone = key >= context, bad = (key >= before) & ((raw[i] & 0x7f80) == 0x7f80) & !gone;
+          wild |= bad;
+          raw[i] = gone | bad ? (unsigned short)0 : raw[i];
+        }
+        *place = raw;
+      }
+    if (__builtin_amdgcn_ballot_w64(wild) != 0 && lane == 0) spoiled[kg][stage] = t + 1;
   };
   int pages[MINE];
   if (t_begin + kg < t_end) {
@@ -168,12 +198,23 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
   }
   const int v_row = CHUNKS * CHUNK + (kq >> 1) * CHUNK + col16 * 16 + (((kq & 1) ^ (col16 >> 3)) * 8);     // .. and of 16 dims' values
 
-  // the queries have arrived (said here, where the compiler sees it: otherwise it waits for them, and with them for the
-  // loads to LDS, before the first product of every turn)
-  __builtin_amdgcn_s_waitcnt(0x0F70);
+  // The queries and masks have arrived: said here, by a use that nothing moves past the loop.  Otherwise the compiler waits for
+  // them, and with them for the tile that has just been asked for, before the first product of every turn (5,376 keys on one
+  // block a CU, 64 columns of 128 dims: 1.05 us a tile).
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) asm volatile("" : "+v"(qv[t][s]));
+    asm volatile("" : "+v"(first_words[t][0]), "+v"(first_words[t][1]));
+  }
   const int turns = (t_end - t_begin + KG - 1) / KG;
   for (int turn = 0; turn < turns; ++turn) {
     const int t = t_begin + turn * KG + kg, stage = turn & 1;
+    if (t < t_end && (t + 1) * KEYS > before) {      // reaches into the step's own entries, or behind them
+      __builtin_amdgcn_s_waitcnt(0x0F70);              // (vmcnt(0))
+      __builtin_amdgcn_sched_barrier(0);
+      tidy(t, stage);
+    }
     // This tile has landed (vmcnt), and the wave's reads of the one before it have ended (lgkmcnt), so that its place may
     // be filled again.
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -185,7 +226,7 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
       }
     }
     if (!works || t >= t_end) continue;      // the same for the whole wave
-#pragma unroll
+#pragma unroll 1
     for (int unit = 0; unit < KEYS / 32; unit += UNITS) {
     const int base = t * KEYS + unit * 32;
     const bf16* st = lds + (kg * 2 + stage) * STAGE + unit * 2 * CHUNK;
@@ -264,43 +305,24 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
           for (int i = 0; i < 4; ++i) p[n][t2][u * 4 + i] = (__bf16)fast_exp2(fmaf(s[n][u][t2][i], scale_log2e, -ref));
         lsum[t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[n][t2], lsum[t2], 0, 0, 0);
       }
-    if (!masked) {
-#pragma unroll
-      for (int n = 0; n < UNITS; ++n)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          const bf16x8 v = *reinterpret_cast<const bf16x8*>(st + n * 2 * CHUNK + v_row + c * 256);
-#pragma unroll
-          for (int t2 = 0; t2 < NT; ++t2) o[c][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[n][t2], o[c][t2], 0, 0, 0);
-        }
-      continue;
-    }
-    // Values behind the context may be anything a reused page still holds: zeros.  Those of the step's entries that are not
-    // finite would reach columns that do not see them: zeros here, and added below for those that do.
-    bool spoiled = false;
 #pragma unroll
     for (int n = 0; n < UNITS; ++n)
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        u16x8 raw = *reinterpret_cast<const u16x8*>(st + n * 2 * CHUNK + v_row + c * 256);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = base + n * 32 + kq * 8 + i;
-          const bool wild = (key >= before) & ((raw[i] & 0x7f80) == 0x7f80), gone = key >= context;
-          spoiled |= wild & !gone;
-          raw[i] = wild | gone ? (unsigned short)0 : raw[i];
-        }
-        const bf16x8 v = __builtin_bit_cast(bf16x8, raw);
+        const bf16x8 v = *reinterpret_cast<const bf16x8*>(st + n * 2 * CHUNK + v_row + c * 256);
 #pragma unroll
         for (int t2 = 0; t2 < NT; ++t2) o[c][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[n][t2], o[c][t2], 0, 0, 0);
       }
-    if (__builtin_amdgcn_ballot_w64(spoiled) != 0) {
+    if (masked && spoiled[kg][stage] == t + 1) {       // (rare: the values are read again from where they are)
+      int rows = page_size;
+      asm volatile("" : "+s"(rows));                   // (nothing of this is worked out ahead of the loop and kept in registers)
 #pragma unroll
       for (int n = 0; n < UNITS; ++n)
         for (int k = 0; k < 32; ++k) {
           const int key = base + n * 32 + k;
           if (key < before || key >= context) continue;
           const int owner = (k >> 3) * 16 + col16;
+          const bf16* from = vt_pages + ((size_t)table[key / rows] * nkv + g) * rows * D + key % rows;
 #pragma unroll
           for (int t2 = 0; t2 < NT; ++t2) {
             float mine = 0.f;
@@ -309,14 +331,14 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
             const float w = __shfl(mine, owner, MS_WAVE);
             const bool see = (__shfl(sees[n][t2], owner, MS_WAVE) >> (k & 7)) & 1u;
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
+            for (int c = 0; c < CT; ++c) {
+              asm volatile("" : "+s"(rows) : : "memory");      // (.. nor the places of all dims at once)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const int dim = c * 16 + kq * 4 + i;
-                const unsigned short raw = __builtin_bit_cast(unsigned short,
-                    st[CHUNKS * CHUNK + (n * 2 + (k >> 4)) * CHUNK + dim * 16 + ((((k >> 3) ^ (dim >> 3)) & 1) * 8) + (k & 7)]);
-                if (see && (raw & 0x7f80u) == 0x7f80u) o[c][t2][i] += w * __uint_as_float((unsigned)raw << 16);
+                const unsigned raw = __builtin_bit_cast(unsigned short, from[(size_t)(c * 16 + kq * 4 + i) * rows]);
+                if (see && (raw & 0x7f80u) == 0x7f80u) o[c][t2][i] += w * __uint_as_float(raw << 16);
               }
+            }
           }
         }
     }
@@ -392,7 +414,7 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
 
 // out[n, h, :] = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the splits that n's request used, a wave to a (token,
 // head): a split's reference and sum to a lane, then every lane its dims of one split after another.
-constexpr int COMBINE_WAVES = 4;
+constexpr int COMBINE_WAVES = 4, AT_ONCE = 8;      // (parts a lane asks for at a time)
 
 template <int D>
 __global__ void __launch_bounds__(COMBINE_WAVES * MS_WAVE)
@@ -424,10 +446,19 @@ tree_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ 
   }
   den = wave_sum(den);
   float acc[DL] = {};
-  for (int s = 0; s < used; ++s) {
-    const float w = __shfl(s < MS_WAVE ? m[0] : m[1], s & (MS_WAVE - 1), MS_WAVE);
+  for (int s0 = 0; s0 < used; s0 += AT_ONCE) {
+    float part[AT_ONCE][DL];
 #pragma unroll
-    for (int e = 0; e < DL; ++e) acc[e] = fmaf(w, part_o[(slot0 + s) * D + min(lane + e * MS_WAVE, D - 1)], acc[e]);
+    for (int s = 0; s < AT_ONCE; ++s)
+#pragma unroll
+      for (int e = 0; e < DL; ++e) part[s][e] = part_o[(slot0 + min(s0 + s, used - 1)) * D + min(lane + e * MS_WAVE, D - 1)];
+#pragma unroll
+    for (int s = 0; s < AT_ONCE; ++s) {
+      const int at = s0 + s;
+      const float w = at < used ? __shfl(at < MS_WAVE ? m[0] : m[1], at & (MS_WAVE - 1), MS_WAVE) : 0.f;
+#pragma unroll
+      for (int e = 0; e < DL; ++e) acc[e] = fmaf(w, part[s][e], acc[e]);
+    }
   }
   const float inv = den != 0.f ? 1.0f / den : 0.f;
 #pragma unroll
@@ -451,6 +482,10 @@ inline long long column_tiles(int n_requests, int n_tokens, int max_q_len, int r
   return std::min((long long)n_tokens * rep / cols + n_requests, ((long long)max_q_len * rep + cols - 1) / cols * n_requests);
 }
 
+inline int page_shift_of(int page_size) {   // log2 of a power of two, else -1
+  return page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size);
+}
+
 template <int D, int WC, int KG, int NT>
 int launch(const Call& a) {
   typedef Shape<D, WC, KG, NT> S;
@@ -467,7 +502,7 @@ int launch(const Call& a) {
   if (tiles > 65535) return MS_UNSUPPORTED;
   tree_attention_mfma_kernel<D, WC, KG, NT><<<dim3(a.nkv, (unsigned)tiles, a.n_splits), dim3(KG * WC * MS_WAVE), S::LDS, a.stream>>>(
       a.q, a.q_stride, a.k, a.vt, a.table, a.table_stride, a.rows, a.q_start, a.ctx, a.tree, a.words, a.out, a.out_stride, a.part_o,
-      a.part_ml, a.nh, a.nkv, a.page_size, a.scale_log2e, one ? 0 : a.n_requests, a.n_splits, a.share / S::KEYS);
+      a.part_ml, a.nh, a.nkv, a.page_size, page_shift_of(a.page_size), a.scale_log2e, one ? 0 : a.n_requests, a.n_splits, a.share / S::KEYS);
   if (a.n_splits > 1) {
     const long long items = (long long)a.n_tokens * a.nh;
     tree_combine_kernel<D><<<dim3((unsigned)((items + COMBINE_WAVES - 1) / COMBINE_WAVES)), dim3(COMBINE_WAVES * MS_WAVE), 0, a.stream>>>(
@@ -476,29 +511,53 @@ int launch(const Call& a) {
   return ms_launch_status();
 }
 
-// Kinds of block: WC waves over columns, KG groups over keys (twice as many below 128 dims), NT tiles of 16 columns a wave.
-struct Kind { int wc, kg, nt; };
-constexpr Kind KINDS[] = {{1, 4, 1}, {2, 2, 1}, {4, 1, 1}, {4, 1, 2}, {4, 2, 1}, {4, 2, 2}};
-constexpr int N_KINDS = sizeof(KINDS) / sizeof(KINDS[0]);
+// Kinds of block: WC waves over columns, KG groups over keys (at 32 and 64 dims F times as many), NT tiles of 16 columns a wave.
+// A block's time is a chain of turns (KG tiles of keys): 5.5 us before and after it, `alone` us a turn with one block on a CU,
+// `pair` where there are two (0: its LDS leaves room for one).
+struct Kind { int wc, kg, nt; double alone, pair; };
+constexpr Kind KINDS[2][4] = {{{1, 8, 1, 0.9, 0.0}, {2, 4, 1, 0.7, 0.9}, {4, 2, 1, 0.9, 1.2}, {4, 1, 2, 1.2, 1.5}},     // 32, 64 dims
+                              {{1, 4, 1, 0.6, 0.0}, {2, 2, 1, 0.7, 0.8}, {4, 1, 1, 1.15, 1.35}, {4, 1, 2, 1.7, 2.1}}};  // 128 dims
 
 }  // namespace
 
-// kind * 65536 + how many times 64 keys a block takes, for a step of these sizes (all bounds); -1: sizes this kernel does
-// not take.
+// kind * 65536 + how many times 64 keys a block takes, for a step of these sizes (all bounds); -1: sizes this kernel does not
+// take.  Narrow kinds share a small step out over the chip, and every block's chain is short; wide ones read the keys less
+// often.  The choice is the least of a model: the chains, as often as all blocks take the chip's room, or the keys at 9 TB/s
+// (what all tiles of columns drew together, from L2s and memory), whichever is longer, and the second kernel (2.8 us, the
+// parts written and read at 3 TB/s).  us measured, the model's choice against the fastest of kinds and shares: 8 tokens of
+// 14 heads of 64 on 2 behind 192 keys 6.3, 6.3 (63 columns a block: 7.9); 32 x 8 behind 700 9.2, 9.2 (12.2); 32 tokens behind
+// 8,000 14.3, 14.3 (21.1 of 128 columns); 28 heads of 128 on 4: 8 x 16 behind 2,000 23.9, 21.8; 32 x 8 behind 1,000 22.8, 22.8
+// (16 columns: 33.7); 40 on 8: 2 x 16 behind 4,000 22.4, 19.9, 4 x 63 behind 16,011 107, 107 (16 columns: 311).
 extern "C" int ms_tree_attention_mfma_plan(int n_requests, int n_tokens, int max_q_len, int max_context_len, int num_heads,
                                            int num_kv_heads, int head_dim, int page_size) {
   if ((head_dim != 32 && head_dim != 64 && head_dim != 128) || page_size <= 0 || page_size % 16) return -1;
   if (n_requests <= 0 || n_tokens <= 0 || max_q_len <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads) return -1;
   const int rep = num_heads / num_kv_heads;
   if ((long long)max_q_len * rep > 0x3fffffffLL) return -1;
-  const int cols = max_q_len * rep;
-  const int kind = cols <= 16 ? 0 : cols <= 32 ? 1 : cols <= 64 ? 2 : 3;
-  const Kind k = KINDS[kind];
-  const long long blocks = column_tiles(n_requests, n_tokens, max_q_len, rep, k.wc * k.nt * 16) * num_kv_heads;
-  const int turn = (k.wc == 4 ? 64 : 32) * k.kg * (head_dim == 128 ? 1 : 2);
-  const long long most = std::max(1, (max_context_len + turn - 1) / turn);
-  const int splits = (int)std::max(1LL, std::min<long long>(std::min<long long>(most, MAX_SPLITS), 2LL * ms_compute_units() / blocks));
-  return kind * 65536 + ((max_context_len + splits - 1) / splits + 63) / 64;
+  const long long context = std::max(1, max_context_len);
+  if (context > 64LL * 65535) return -1;
+  const double cus = ms_compute_units(), cols = (double)n_tokens * rep;
+  double best = 0.0;
+  int choice = -1;
+  for (int kind = 0; kind < 4; ++kind) {
+    const Kind k = KINDS[head_dim == 128][kind];
+    const int width = k.wc * k.nt * 16, turn = (k.wc == 4 ? 64 : 32) * k.kg;
+    // a request ends in half a tile on average, unless one tile is all it has
+    const double tiles = ((long long)max_q_len * rep <= width ? (double)n_requests : cols / width + 0.5 * n_requests) * num_kv_heads;
+    const double draws = tiles * context * head_dim * 4 / 9e6;
+    for (const int n : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128}) {
+      const long long share = ((context + n - 1) / n + turn - 1) / turn * turn, turns = share / turn, splits = (context + share - 1) / share;
+      if (splits > MAX_SPLITS) continue;
+      const double blocks = tiles * splits;
+      const bool pairs = k.pair > 0.0 && blocks > cus;
+      const double rounds = std::max(1.0, blocks / (pairs ? 2.0 * cus : cus));
+      double us = 5.5 + std::max(turns * (pairs ? k.pair : k.alone) * rounds, draws);
+      if (splits > 1) us += 2.8 + (double)n_tokens * num_heads * splits * (head_dim + 2) * 8 / 3e6;
+      if (choice < 0 || us < best) { best = us; choice = kind * 65536 + (int)(share / 64); }
+      if (n > 1 && turns == 1) break;
+    }
+  }
+  return choice;
 }
 
 // part_o: float [n_tokens, num_heads, n_splits, head_dim], part_ml: float [n_tokens, num_heads, n_splits, 2] (null with one).
@@ -522,8 +581,7 @@ extern "C" int ms_tree_attention_mfma(const void* q, long long q_stride, const v
                   (const unsigned*)tree, (bf16*)out, (float*)part_o, (float*)part_ml, (size_t)q_stride, (size_t)out_stride, table_stride,
                   words, n_requests, n_tokens, max_q_len, num_heads, num_kv_heads, page_size, n_splits, share, scale * 1.4426950408889634f, stream};
 #define GO(D, F) switch (kind) { case 0: return launch<D, 1, 4 * F, 1>(a); case 1: return launch<D, 2, 2 * F, 1>(a); \
-                                 case 2: return launch<D, 4, F, 1>(a); case 3: return launch<D, 4, 1, 2>(a); \
-                                 case 4: return launch<D, 4, 2 * F, 1>(a); case 5: return launch<D, 4, 2, 2>(a); }
+                                 case 2: return launch<D, 4, F, 1>(a); case 3: return launch<D, 4, 1, 2>(a); }
   if (head_dim == 32) GO(32, 2);
   if (head_dim == 64) GO(64, 2);
   if (head_dim == 128) GO(128, 1);
