@@ -236,8 +236,9 @@ long long ms_sample_workspace_bytes(int n_rows);
 int ms_sample(const float* logits, long long ld, int n_rows, int vocab, const float* temperature, const int* top_k,
               const float* top_p, const unsigned long long* seeds, const int* draw_index, int* out, void* workspace,
               int use_top_k, int use_top_p, hipStream_t stream);
-// out [n_rows, vocab] (row stride out_ld): the distributions ms_sample would draw from; arguments and workspace as there.
-// out must not be logits.
+// out [n_rows, vocab] (row stride out_ld): the distributions ms_sample would draw from; arguments as there.  out must not be
+// logits.  workspace: ms_probabilities_workspace_bytes(n_rows) bytes of device memory (any contents).
+long long ms_probabilities_workspace_bytes(int n_rows);
 int ms_probabilities(const float* logits, long long ld, int n_rows, int vocab, const float* temperature, const int* top_k,
                      const float* top_p, float* out, long long out_ld, void* workspace, int use_top_k, int use_top_p,
                      hipStream_t stream);

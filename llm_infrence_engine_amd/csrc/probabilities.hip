@@ -1,0 +1,515 @@
+// The distributions that tokens are drawn from, whole: out[r, i] = e^(s_i - max) / sum over the kept e^(s_j - max) for the kept
+// i of row r and 0 for the others, s = logits / temperature.  What is kept is decided as in csrc/sampling.hip, with masses e^(s -
+// max) in fixed point whose sums are exact; a row without temperature is a one at its first maximum.
+//
+// The work is two readings of the logits and one writing; the rest is to find the floor, the smallest value kept, in few
+// launches and without a sort.  A row is spread over n_chunks blocks; with `target` = top_p times the mass that top-k keeps:
+//   1 every chunk's maximum; with a top-k also the maxima of groups of a wave's lanes (as many groups as four times k or so)
+//   2 top-k: the k-th largest group maximum is no larger than the k-th largest value, and only a few more than k values are above
+//     it (50 of 384 groups: 54 expected): these are collected as candidates, those equal to it counted
+//     top-p alone: every chunk's mass, and a histogram of masses by the distance from the maximum (1/128 wide, 2,048 of them), in
+//     float: its sums depend on the order, so it only says where to look
+//   3 top-p alone: the values of the histogram's bin in which the target falls, and of its neighbours, are the candidates;
+//     the mass above them is summed up exactly
+//   4 a thread to a candidate: count and mass of the larger ones say whether it is kept, the least kept one is the floor; then
+//     every block writes its chunk
+// What the candidates cannot decide (more than MAX_CANDIDATES of them, a k beyond half the groups, a target outside the
+// candidates' masses) every block of the row finds by itself with a radix descent over the whole row: right for any input, and
+// slow (a row of 151,936: about 100 us).
+#include "sampling.h"
+#include "api.h"
+#include <algorithm>
+
+// A scaled logit is rounded to a float before anything else is done with it: its key, its mass and its probability are those of one
+// number, wherever they are worked out (a product joined with the subtraction of the maximum is another one).
+#pragma clang fp contract(off)
+
+namespace {
+
+constexpr int MAX_CHUNKS = 32, WAVES = THREADS / MS_WAVE;
+constexpr int MAX_CANDIDATES = THREADS;
+constexpr int BINS = 2048;
+constexpr float BINS_A_UNIT = 128.f;
+
+struct RowWork {                       // one per row, in the workspace the caller brings
+  unsigned chunk_max[MAX_CHUNKS];      // key of the largest scaled logit of every chunk (no temperature: the largest itself)
+  unsigned n_candidates, n_ties;       // ties: values equal to the bound
+  unsigned bound;                      // top-k: every value above it is a candidate
+  int bin;                             // top-p alone: the middle bin of the candidates, < 0: none
+  unsigned long long chunk_mass[MAX_CHUNKS];    // (no temperature: where the largest stands)
+  unsigned long long chunk_above[MAX_CHUNKS];   // mass of the values above the candidates'
+  unsigned candidates[MAX_CANDIDATES];          // keys
+  float hist[BINS];
+  unsigned groups[MAX_CHUNKS * WAVES * 4];
+};
+
+// What a row asks for, and how its candidates are found.
+struct RowPlan {
+  float inv_t, p;
+  int k;                 // 0: no top-k
+  bool greedy, use_p;
+  bool all;              // few enough values: all are candidates
+  int groups;            // of a wave (0: none, or too few for k)
+};
+
+__device__ __forceinline__ RowPlan plan_of(const float* temperature, const int* top_k, const float* top_p, int r, int V, int n_chunks) {
+  RowPlan a;
+  const float T = temperature[r];
+  a.greedy = !(T > 0.f);
+  a.inv_t = 1.0f / T;
+  const int k = top_k ? top_k[r] : 0;
+  a.k = k > 0 && k < V ? k : 0;
+  a.p = top_p ? top_p[r] : 1.f;
+  a.use_p = a.p < 1.f;
+  a.all = V <= MAX_CANDIDATES;
+  const int waves = n_chunks * WAVES;
+  a.groups = !a.k || a.all ? 0 : 4LL * a.k <= waves ? 1 : 4LL * a.k <= 2 * waves ? 2 : 2LL * a.k <= 4 * waves ? 4 : 0;
+  return a;
+}
+
+// A row in quads of four values on 16 bytes: quad q of a row that begins `lead` values behind such a place holds its values
+// 4 q - lead .. + 3.
+__device__ __forceinline__ int lead_of(const float* row) { return (int)(((uintptr_t)row >> 2) & 3); }
+
+__device__ __forceinline__ void quad_range(const float* row, int V, int n_chunks, int c, int* begin, int* end) {
+  const int quads = (lead_of(row) + V + 3) / 4, len = (quads + n_chunks - 1) / n_chunks;
+  *begin = min(quads, c * len);
+  *end = min(quads, *begin + len);
+}
+
+// f(i, v): the values i .. i + 3 of this thread's quads begin .. end - 1 (places outside the row: NaN), four quads under way at a
+// time and none behind a condition; the quads at a row's ends, which may lie in part outside of it, value by value.
+template <typename F>
+__device__ __forceinline__ void for_quads(const float* __restrict__ row, int V, int begin, int end, F f) {
+  constexpr int AT_ONCE = 4;
+  const int lead = lead_of(row), first = lead ? 1 : 0, last = (lead + V) / 4 - 1;      // the whole quads
+  const float* base = row - lead;
+  for (int q0 = begin + threadIdx.x; q0 < end; q0 += AT_ONCE * THREADS) {
+    float4 v[AT_ONCE];
+    if (first <= last) {
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) v[j] = *reinterpret_cast<const float4*>(base + 4 * (size_t)min(max(q0 + j * THREADS, first), last));
+    }
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int q = q0 + j * THREADS;
+      if (q >= end) break;
+      if (q < first || q > last) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = 4 * q - lead + i;
+          e[i] = at >= 0 && at < V ? row[at] : __builtin_nanf("");
+        }
+        v[j] = make_float4(e[0], e[1], e[2], e[3]);
+      }
+      f(4 * q - lead, v[j]);
+    }
+  }
+}
+template <typename F>
+__device__ __forceinline__ void for_values(const float* __restrict__ row, int V, int begin, int end, F f) {
+  for_quads(row, V, begin, end, [&](int, const float4& v) { f(v.x); f(v.y); f(v.z); f(v.w); });
+}
+
+__device__ unsigned long long block_sum_u64(unsigned long long v, unsigned long long* red) {
+  for (int o = MS_WAVE / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
+  __syncthreads();
+  if ((threadIdx.x & (MS_WAVE - 1)) == 0) red[threadIdx.x / MS_WAVE] = v;
+  __syncthreads();
+  unsigned long long s = 0;
+  for (int w = 0; w < WAVES; ++w) s += red[w];
+  return s;
+}
+
+__device__ __forceinline__ unsigned largest_key(const RowWork& w, int n_chunks) {
+  unsigned best = 0;
+  for (int c = 0; c < n_chunks; ++c) best = max(best, w.chunk_max[c]);
+  return best;
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+__device__ __forceinline__ int bin_of(float s, float zmax) {      // BINS: beyond them, or NaN
+  const float x = (zmax - s) * BINS_A_UNIT;
+  return x < (float)BINS ? (int)x : BINS;
+}
+
+// ---- 1
+__global__ void __launch_bounds__(THREADS)
+probabilities_max_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
+                         const int* __restrict__ top_k, const float* __restrict__ top_p, RowWork* __restrict__ work, int n_chunks) {
+  __shared__ unsigned red[WAVES];
+  __shared__ MaxIdx red_mi[WAVES];
+  const int r = blockIdx.y, c = blockIdx.x, lane = threadIdx.x & (MS_WAVE - 1), wave = threadIdx.x / MS_WAVE;
+  RowWork& w = work[r];
+  const RowPlan a = plan_of(temperature, top_k, top_p, r, V, n_chunks);
+  const float* row = logits + (size_t)r * ld;
+  int begin, end;
+  quad_range(row, V, n_chunks, c, &begin, &end);
+  if (a.greedy) {
+    MaxIdx best = {-INFINITY, 0x7fffffff};
+    for_quads(row, V, begin, end, [&](int i, const float4& v) {
+      best = better(best, MaxIdx{v.x, i});
+      best = better(best, MaxIdx{v.y, i + 1});
+      best = better(best, MaxIdx{v.z, i + 2});
+      best = better(best, MaxIdx{v.w, i + 3});
+    });
+    for (int o = MS_WAVE / 2; o > 0; o >>= 1) best = better(best, MaxIdx{__shfl_xor(best.v, o, MS_WAVE), __shfl_xor(best.i, o, MS_WAVE)});
+    if (lane == 0) red_mi[wave] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int k = 1; k < WAVES; ++k) best = better(best, red_mi[k]);
+      w.chunk_max[c] = __float_as_uint(best.v);
+      w.chunk_mass[c] = (unsigned)best.i;
+    }
+    return;
+  }
+  if (c == 0 && threadIdx.x == 0) { w.n_candidates = 0u; w.n_ties = 0u; w.bin = -1; w.bound = 0u; }
+  if (threadIdx.x == 0) { w.chunk_mass[c] = 0ull; w.chunk_above[c] = 0ull; }
+  if (a.use_p && !a.k && !a.all)
+    for (int i = c * THREADS + threadIdx.x; i < BINS; i += n_chunks * THREADS) w.hist[i] = 0.f;
+  unsigned best = 0;
+  for_values(row, V, begin, end, [&](float v) {
+    const float s = v * a.inv_t;
+    best = s == s ? max(best, order_key(s)) : best;     // NaN never wins
+  });
+  for (int o = 1; o < MS_WAVE; o <<= 1) {
+    if (a.groups && o * a.groups == MS_WAVE && (lane & (o - 1)) == 0) w.groups[(c * WAVES + wave) * a.groups + lane / o] = best;
+    best = max(best, (unsigned)__shfl_xor((int)best, o, MS_WAVE));
+  }
+  if (lane == 0) {
+    red[wave] = best;
+    if (a.groups == 1) w.groups[c * WAVES + wave] = best;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < WAVES; ++k) best = max(best, red[k]);
+    w.chunk_max[c] = best;
+  }
+}
+
+// ---- 2
+__global__ void __launch_bounds__(THREADS)
+probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
+                             const int* __restrict__ top_k, const float* __restrict__ top_p, RowWork* __restrict__ work, int n_chunks) {
+  __shared__ unsigned long long red[WAVES];
+  __shared__ unsigned keys[MAX_CHUNKS * WAVES * 4];
+  __shared__ unsigned bound_sm;
+  const int r = blockIdx.y, c = blockIdx.x;
+  RowWork& w = work[r];
+  const RowPlan a = plan_of(temperature, top_k, top_p, r, V, n_chunks);
+  if (a.greedy) return;
+  const float* row = logits + (size_t)r * ld;
+  int begin, end;
+  quad_range(row, V, n_chunks, c, &begin, &end);
+  const float zmax = key_value(largest_key(w, n_chunks));
+  if (!finite(zmax)) return;      // no mass: the last kernel puts a one where the greedy choice stands
+  if ((a.k || a.use_p) && a.all) {
+    for_values(row, V, begin, end, [&](float v) {
+      const float s = v * a.inv_t;
+      if (s == s) w.candidates[atomicAdd(&w.n_candidates, 1u)] = order_key(s);
+    });
+    return;
+  }
+  if (a.k) {
+    if (!a.groups) return;
+    const int n = n_chunks * WAVES * a.groups;
+    for (int i = threadIdx.x; i < n; i += THREADS) keys[i] = w.groups[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += THREADS) {      // the k-th largest of them
+      const unsigned mine = keys[i];
+      int above = 0, equal = 0;
+      for (int j = 0; j < n; j += 4) {                    // (n is a multiple of 16)
+        const uint4 o = *reinterpret_cast<const uint4*>(&keys[j]);
+        above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+        equal += (o.x == mine) + (o.y == mine) + (o.z == mine) + (o.w == mine);
+      }
+      if (above < a.k && a.k <= above + equal) bound_sm = mine;      // (all who find it find the same)
+    }
+    __syncthreads();
+    const unsigned bound = bound_sm;
+    unsigned ties = 0;
+    for_values(row, V, begin, end, [&](float v) {
+      const float s = v * a.inv_t;
+      if (!(s == s)) return;
+      const unsigned key = order_key(s);
+      if (key > bound) {
+        const unsigned at = atomicAdd(&w.n_candidates, 1u);
+        if (at < MAX_CANDIDATES) w.candidates[at] = key;
+      }
+      ties += key == bound;
+    });
+    const unsigned long long all = block_sum_u64(ties, red);
+    if (threadIdx.x == 0) {
+      if (all) atomicAdd(&w.n_ties, (unsigned)all);
+      if (c == 0) w.bound = bound;
+    }
+    return;
+  }
+  unsigned long long mine = 0;
+  if (!a.use_p) {
+    for_values(row, V, begin, end, [&](float v) {
+      const float s = v * a.inv_t;
+      if (s == s) mine += fixed_mass(s, zmax);
+    });
+  } else {
+    float* hist = reinterpret_cast<float*>(keys);      // BINS of them
+    static_assert(sizeof(keys) >= BINS * sizeof(float), "the histogram fits");
+    for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0.f;
+    __syncthreads();
+    for_values(row, V, begin, end, [&](float v) {
+      const float s = v * a.inv_t;
+      if (!(s == s)) return;
+      const float e = expf(s - zmax);
+      mine += (unsigned long long)(e * (float)(1ull << FIX_PLACES));      // (fixed_mass)
+      const int bin = bin_of(s, zmax);
+      if (bin < BINS) unsafeAtomicAdd(&hist[bin], e);
+    });
+    __syncthreads();
+    for (int i = threadIdx.x; i < BINS; i += THREADS)
+      if (hist[i] != 0.f) unsafeAtomicAdd(&w.hist[i], hist[i]);
+  }
+  mine = block_sum_u64(mine, red);
+  if (threadIdx.x == 0) w.chunk_mass[c] = mine;
+}
+
+__device__ __forceinline__ unsigned long long target_of(float p, unsigned long long total) {      // as the sampler has it
+  const unsigned long long target = (unsigned long long)((double)p * (double)total);
+  return target > 0 ? target : 1ull;
+}
+
+// ---- 3
+__global__ void __launch_bounds__(THREADS)
+probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
+                          const int* __restrict__ top_k, const float* __restrict__ top_p, RowWork* __restrict__ work, int n_chunks) {
+  __shared__ unsigned long long red[WAVES];
+  __shared__ float wave_sum_sm[WAVES];
+  __shared__ int found;
+  const int r = blockIdx.y, c = blockIdx.x, lane = threadIdx.x & (MS_WAVE - 1), wave = threadIdx.x / MS_WAVE;
+  RowWork& w = work[r];
+  const RowPlan a = plan_of(temperature, top_k, top_p, r, V, n_chunks);
+  if (a.greedy || a.k || !a.use_p || a.all) return;
+  const float zmax = key_value(largest_key(w, n_chunks));
+  if (!finite(zmax)) return;
+  unsigned long long total = 0;
+  for (int k = 0; k < n_chunks; ++k) total += w.chunk_mass[k];
+  const float target = (float)((double)target_of(a.p, total) / (double)(1ull << FIX_PLACES));
+  // the first bin at which the running mass reaches the target; a thread owns two bins
+  const float h0 = w.hist[2 * threadIdx.x], h1 = w.hist[2 * threadIdx.x + 1];
+  float run = h0 + h1;
+  for (int o = 1; o < MS_WAVE; o <<= 1) {
+    const float v = __shfl_up(run, o, MS_WAVE);
+    if (lane >= o) run += v;
+  }
+  if (lane == MS_WAVE - 1) wave_sum_sm[wave] = run;
+  if (threadIdx.x == 0) found = BINS;
+  __syncthreads();
+  for (int k = 0; k < wave; ++k) run += wave_sum_sm[k];
+  if (run >= target) atomicMin(&found, run - h1 >= target ? 2 * (int)threadIdx.x : 2 * (int)threadIdx.x + 1);
+  __syncthreads();
+  // (sums of floats may fall short of a target that is nearly everything: the last bin that has any would be no surer)
+  if (found >= BINS) return;
+  const int lo = found - 1, hi = found + 1;
+  if (c == 0 && threadIdx.x == 0) w.bin = found;
+  const float* row = logits + (size_t)r * ld;
+  int begin, end;
+  quad_range(row, V, n_chunks, c, &begin, &end);
+  unsigned long long above = 0;
+  for_values(row, V, begin, end, [&](float v) {
+    const float s = v * a.inv_t;
+    if (!(s == s)) return;
+    const int bin = bin_of(s, zmax);
+    if (bin < lo) {
+      above += fixed_mass(s, zmax);
+    } else if (bin <= hi && bin < BINS) {
+      const unsigned at = atomicAdd(&w.n_candidates, 1u);
+      if (at < MAX_CANDIDATES) w.candidates[at] = order_key(s);
+    }
+  });
+  above = block_sum_u64(above, red);
+  if (threadIdx.x == 0) w.chunk_above[c] = above;
+}
+
+struct Kept { unsigned floor; unsigned long long mass; };
+
+// The floor by a radix descent of this block over the whole row, and the mass of what is kept.
+__device__ Kept descend(const float* __restrict__ row, int V, const RowPlan& a, float zmax, unsigned* lc, unsigned long long* lm) {
+  const int quads = (lead_of(row) + V + 3) / 4, lane = threadIdx.x & (MS_WAVE - 1);
+  // the key at which the running count (or mass) from the top reaches `need`, among keys of at least `least`; with the mass upto it
+  auto search = [&](bool by_mass, unsigned long long need, unsigned least) {
+    unsigned digits = 0;
+    unsigned long long above = 0, mass = 0;
+    for (int level = 1; level <= 3; ++level) {
+      const int shift = level_shift(level), bins = level_bins(level);
+      __syncthreads();
+      for (int i = threadIdx.x; i < bins; i += THREADS) { lc[i] = 0u; lm[i] = 0ull; }
+      __syncthreads();
+      for_values(row, V, 0, quads, [&](float v) {
+        const float s = v * a.inv_t;
+        const unsigned key = order_key(s);
+        const bool in = s == s && key >= least && (level == 1 || (key >> (shift + (level == 2 ? 11 : 10))) == digits);
+        const int bin = (int)((key >> shift) & (unsigned)(bins - 1));
+        unsigned long long m = in ? fixed_mass(s, zmax) : 0ull;
+        const unsigned long long who = __ballot(in);
+        if (!who) return;
+        const int leader = __builtin_ctzll(who);
+        if (__ballot(in && bin != __shfl(bin, leader, MS_WAVE)) == 0 && __builtin_popcountll(__ballot(true)) == MS_WAVE) {
+          // one bin for all of them, as in rows of few different values: one addition for the wave
+          for (int o = MS_WAVE / 2; o > 0; o >>= 1) m += __shfl_xor(m, o, MS_WAVE);
+          if (lane == leader) { atomicAdd(&lc[bin], (unsigned)__builtin_popcountll(who)); atomicAdd(&lm[bin], m); }
+        } else if (in) {
+          atomicAdd(&lc[bin], 1u);
+          atomicAdd(&lm[bin], m);
+        }
+      });
+      __syncthreads();
+      const Found f = first_bin_reaching(lc, lm, bins, by_mass, need - above);
+      digits = level == 1 ? (unsigned)f.bin : (digits << (level == 2 ? 11 : 10)) | (unsigned)f.bin;
+      above += by_mass ? f.mass_above : f.count_above;
+      mass += f.mass_above + (level == 3 ? f.mass_in : 0ull);
+    }
+    return Kept{digits, mass};
+  };
+  Kept k = search(false, a.k ? (unsigned long long)a.k : ~0ull >> 1, 0u);
+  if (!a.k) k.floor = 0u;
+  if (!a.use_p) return k;
+  return search(true, target_of(a.p, k.mass), k.floor);
+}
+
+// ---- 4
+__global__ void __launch_bounds__(THREADS)
+probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
+                           const int* __restrict__ top_k, const float* __restrict__ top_p, const RowWork* __restrict__ work,
+                           int n_chunks, float* __restrict__ out, size_t out_ld) {
+  __shared__ MaxIdx red_mi[WAVES];
+  __shared__ unsigned long long red[WAVES];
+  __shared__ unsigned keys[RADIX_BINS];
+  __shared__ unsigned long long masses[RADIX_BINS];
+  __shared__ unsigned floor_sm;
+  const int r = blockIdx.y, c = blockIdx.x;
+  const RowWork& w = work[r];
+  const RowPlan a = plan_of(temperature, top_k, top_p, r, V, n_chunks);
+  const float* row = logits + (size_t)r * ld;
+  float* to = out + (size_t)r * out_ld;
+  int begin, end;
+  quad_range(row, V, n_chunks, c, &begin, &end);
+  // four values of the row's quads at a time where out's rows lie as the logits' do
+  const bool alike = lead_of(row) == lead_of(to);
+  auto store = [&](int i, const float4& v) {
+    if (alike && i >= 0 && i + 3 < V) {
+      *reinterpret_cast<float4*>(to + i) = v;
+    } else {
+      const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j >= 0 && i + j < V) to[i + j] = e[j];
+    }
+  };
+  const unsigned top = a.greedy ? 0u : largest_key(w, n_chunks);
+  const float zmax = a.greedy ? 0.f : key_value(top);
+  int one = -1;
+  if (a.greedy) {
+    MaxIdx best = {-INFINITY, 0x7fffffff};
+    for (int k = 0; k < n_chunks; ++k) best = better(best, MaxIdx{__uint_as_float(w.chunk_max[k]), (int)w.chunk_mass[k]});
+    one = best.i == 0x7fffffff ? 0 : best.i;
+  } else if (!finite(zmax)) {
+    const MaxIdx best = block_argmax(row, 0, V, red_mi);
+    one = best.i == 0x7fffffff ? 0 : best.i;
+  }
+  if (one >= 0) {
+    const int lead = lead_of(row);
+    for (int q = begin + threadIdx.x; q < end; q += THREADS) {
+      const int i = 4 * q - lead;
+      store(i, make_float4(i == one ? 1.f : 0.f, i + 1 == one ? 1.f : 0.f, i + 2 == one ? 1.f : 0.f, i + 3 == one ? 1.f : 0.f));
+    }
+    return;
+  }
+
+  Kept kept = {0u, 0ull};
+  if (!a.k && !a.use_p) {
+    for (int k = 0; k < n_chunks; ++k) kept.mass += w.chunk_mass[k];
+  } else {
+    const int n = (int)w.n_candidates;
+    bool known = n <= MAX_CANDIDATES && (a.all || (a.k ? a.groups > 0 : w.bin >= 0));
+    if (known) {
+      // a thread to a candidate; values equal to the bound are one more, as often as they were counted
+      const bool tied = a.k && !a.all;
+      const unsigned ties = tied ? w.n_ties : 0u;
+      const unsigned long long tie_mass = tied ? fixed_mass(key_value(w.bound), zmax) : 0ull;
+      unsigned mine = 0u;
+      unsigned long long mass = 0ull, above_all = 0ull;
+      if ((int)threadIdx.x < n) {
+        mine = w.candidates[threadIdx.x];
+        mass = fixed_mass(key_value(mine), zmax);
+        keys[threadIdx.x] = mine;
+        masses[threadIdx.x] = mass;
+      }
+      if (!a.k && !a.all)
+        for (int k = 0; k < n_chunks; ++k) above_all += w.chunk_above[k];
+      if (threadIdx.x == 0) floor_sm = 0xffffffffu;
+      __syncthreads();
+      unsigned count = 0;
+      unsigned long long larger = above_all;
+      if ((int)threadIdx.x < n)
+        for (int j = 0; j < n; ++j)
+          if (keys[j] > mine) { ++count; larger += masses[j]; }
+      // what top-k keeps (the bound's values are kept if fewer than k are larger)
+      const bool in_k = (int)threadIdx.x < n && (!a.k || count < (unsigned)a.k);
+      const bool ties_in_k = ties > 0 && (unsigned)n < (unsigned)a.k;
+      unsigned long long total = above_all + block_sum_u64(in_k ? mass : 0ull, red) + (ties_in_k ? ties * tie_mass : 0ull);
+      bool in = in_k, ties_in = ties_in_k;
+      if (a.use_p) {
+        unsigned long long whole = total;
+        if (!a.k && !a.all) {
+          whole = 0;
+          for (int k = 0; k < n_chunks; ++k) whole += w.chunk_mass[k];
+        }
+        const unsigned long long target = target_of(a.p, whole);
+        known = above_all < target && total >= target;      // (it falls among the candidates)
+        in = in_k && larger < target;
+        const unsigned long long all_in = block_sum_u64(in_k ? mass : 0ull, red);
+        ties_in = ties_in_k && all_in < target;
+        total = above_all + block_sum_u64(in ? mass : 0ull, red) + (ties_in ? ties * tie_mass : 0ull);
+      }
+      if (in) atomicMin(&floor_sm, mine);
+      if (ties_in && threadIdx.x == 0) atomicMin(&floor_sm, w.bound);
+      __syncthreads();
+      kept = Kept{floor_sm, total};
+    }
+    if (!known) kept = descend(row, V, a, zmax, keys, masses);
+  }
+  const float inv = (float)((double)(1ull << FIX_PLACES) / (double)kept.mass);
+  for_quads(row, V, begin, end, [&](int i, const float4& v) {
+    auto value = [&](float x) {
+      const float s = x * a.inv_t;
+      return s == s && order_key(s) >= kept.floor ? expf(s - zmax) * inv : 0.f;
+    };
+    store(i, make_float4(value(v.x), value(v.y), value(v.z), value(v.w)));
+  });
+}
+
+}  // namespace
+
+// Bytes of workspace ms_probabilities needs for n_rows rows (any contents: the first kernel makes it ready).
+extern "C" long long ms_probabilities_workspace_bytes(int n_rows) { return (long long)sizeof(RowWork) * (n_rows > 0 ? n_rows : 0); }
+
+// out[r, :] = the distribution ms_sample would draw row r's token from; arguments as there.
+extern "C" int ms_probabilities(const float* logits, long long ld, int n_rows, int vocab, const float* temperature,
+                                const int* top_k, const float* top_p, float* out, long long out_ld, void* workspace,
+                                int use_top_k, int use_top_p, hipStream_t stream) {
+  if (n_rows <= 0) return MS_OK;
+  if (vocab <= 0 || ld < vocab || out_ld < vocab || n_rows > 65535 || temperature == nullptr) return MS_BAD_ARG;
+  if (workspace == nullptr || ((uintptr_t)workspace % 8)) return MS_BAD_ARG;
+  RowWork* work = (RowWork*)workspace;
+  if (!use_top_k) top_k = nullptr;
+  if (!use_top_p) top_p = nullptr;
+  // about two blocks a CU
+  int n_chunks = (2 * ms_compute_units() + n_rows - 1) / n_rows;
+  n_chunks = std::max(1, std::min(std::min(n_chunks, MAX_CHUNKS), (vocab + 2047) / 2048));
+  const dim3 grid(n_chunks, n_rows), block(THREADS);
+  probabilities_max_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks);
+  probabilities_collect_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks);
+  if (top_p) probabilities_near_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks);
+  probabilities_write_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks, out, (size_t)out_ld);
+  return ms_launch_status();
+}

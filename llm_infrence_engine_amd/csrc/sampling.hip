@@ -6,19 +6,12 @@
 // The k-th value and the top-p threshold are found over an order-preserving integer image of the floats, by a
 // radix descent that spreads every row over many blocks (see below), so no sort is needed.  The uniform number
 // of a draw is Philox4x32-10(seed, draw index): the same seed and index give the same token.
-#include "common.h"
+#include "sampling.h"
 #include "api.h"
 #include <algorithm>
 #include <mutex>
 
 namespace {
-
-constexpr int THREADS = 1024;
-
-__device__ __forceinline__ unsigned order_key(float f) {  // a < b  <=>  key(a) < key(b)
-  const unsigned u = __float_as_uint(f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
 
 __device__ __forceinline__ unsigned mulhi32(unsigned a, unsigned b) { return __umulhi(a, b); }
 
@@ -35,45 +28,6 @@ __device__ float philox_uniform(unsigned long long seed, unsigned counter) {
   return (float)(c0 >> 8) * (1.0f / 16777216.0f);  // [0, 1)
 }
 
-struct MaxIdx { float v; int i; };
-
-__device__ __forceinline__ MaxIdx better(MaxIdx a, MaxIdx b) {  // larger value, then smaller index; NaN never wins
-  if (b.v > a.v || (b.v == a.v && b.i < a.i)) return b;
-  return a;
-}
-
-// f(i, row[i]) for this thread's share of row[begin..end), in no particular order; eight loads under way at a time (64 rows of
-// 151,936 with top-k and top-p, 19 logits a thread: 143 -> 124 us; up to 16 rows, at most 10 logits a thread, no difference).
-template <typename F>
-__device__ __forceinline__ void for_share(const float* __restrict__ row, int begin, int end, F f) {
-  constexpr int AT_ONCE = 8;
-  for (int base = begin + threadIdx.x; base < end; base += AT_ONCE * THREADS) {
-    float v[AT_ONCE];
-#pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j) v[j] = row[min(base + j * THREADS, end - 1)];
-#pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j)
-      if (base + j * THREADS < end) f(base + j * THREADS, v[j]);
-  }
-}
-
-// The first maximum of row[begin..end); index 0x7fffffff: there is none but NaN.
-__device__ MaxIdx block_argmax(const float* __restrict__ row, int begin, int end, MaxIdx* red) {
-  MaxIdx best = {-INFINITY, 0x7fffffff};
-  for_share(row, begin, end, [&](int i, float v) { best = better(best, MaxIdx{v, i}); });
-  for (int o = MS_WAVE / 2; o > 0; o >>= 1) {
-    MaxIdx other = {__shfl_xor(best.v, o, MS_WAVE), __shfl_xor(best.i, o, MS_WAVE)};
-    best = better(best, other);
-  }
-  const int lane = threadIdx.x & (MS_WAVE - 1), wave = threadIdx.x / MS_WAVE;
-  __syncthreads();
-  if (lane == 0) red[wave] = best;
-  __syncthreads();
-  MaxIdx r = red[0];
-  for (int w = 1; w < (int)(blockDim.x / MS_WAVE); ++w) r = better(r, red[w]);
-  return r;
-}
-
 // ------------------------------------------------------------------------------------------------
 // The draw.  A row is spread over n_chunks blocks, and the two thresholds are found by a radix descent over the
 // 32-bit keys in three levels (11 + 11 + 10 bits) instead of a bitwise search of 32 + 32 passes by one block:
@@ -88,10 +42,8 @@ __device__ MaxIdx block_argmax(const float* __restrict__ row, int begin, int end
 // do not depend on the order in which blocks add them (integer atomics), and every kernel that works one out
 // again gets the same bits.  Last, the kept mass of every chunk and one block per row that walks the chunk
 // where u * total falls, in index order.
-constexpr int RADIX_BINS = 2048;
 constexpr int MAX_CHUNKS = 64;
 constexpr int N_HIST = 5;            // levels 1 to 3 of the top-k descent, levels 2 and 3 of the top-p descent
-constexpr int FIX_PLACES = 44;
 
 struct RowWork {                     // one per row, in the workspace the caller brings
   // Every field is written by one kernel (block 0 of the row) and read by later kernels only.
@@ -110,71 +62,10 @@ struct RowWork {                     // one per row, in the workspace the caller
   unsigned long long mass[N_HIST][RADIX_BINS];
 };
 
-__device__ __forceinline__ unsigned long long fixed_mass(float s, float zmax) {
-  return (unsigned long long)(expf(s - zmax) * (float)(1ull << FIX_PLACES));   // at most 2^44: exact for a float
-}
-
-__device__ __forceinline__ float key_value(unsigned key) {   // the float whose key this is
-  return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
-}
-
 __device__ __forceinline__ unsigned row_max_key(const RowWork& w, int n_chunks) {
   unsigned best = 0;
   for (int c = 0; c < n_chunks; ++c) best = max(best, w.chunk_max[c]);
   return best;
-}
-
-__device__ __forceinline__ int level_shift(int level) { return level == 1 ? 21 : (level == 2 ? 10 : 0); }
-__device__ __forceinline__ int level_bins(int level) { return level == 3 ? 1024 : RADIX_BINS; }
-
-struct Found { int bin; unsigned long long count_above, mass_above, count_in, mass_in; };
-
-// The first bin, from the top, at which the running count (by_mass = false) or mass of the bins so far reaches
-// `need`; with it the count and mass of the bins above it and of the bin itself.  If none does, the lowest
-// bin that holds anything (or bin 0).  Every thread of the block calls this and gets the same answer.
-__device__ Found first_bin_reaching(const unsigned* __restrict__ count, const unsigned long long* __restrict__ mass,
-                                    int bins, bool by_mass, unsigned long long need) {
-  __shared__ unsigned long long wave_c[THREADS / MS_WAVE], wave_m[THREADS / MS_WAVE];
-  __shared__ Found found;
-  __shared__ int lowest;
-  const int t = threadIdx.x, lane = t & (MS_WAVE - 1), wave = t / MS_WAVE;
-  // thread t owns bins hi and hi - 1, hi = bins - 1 - 2 t: thread 0 the two topmost
-  const int hi = bins - 1 - 2 * t;
-  unsigned long long c[2] = {0, 0}, m[2] = {0, 0};
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    if (hi - j >= 0) { c[j] = count[hi - j]; m[j] = mass[hi - j]; }
-  unsigned long long sc = c[0] + c[1], sm = m[0] + m[1];     // inclusive scan over threads, from the top
-  for (int o = 1; o < MS_WAVE; o <<= 1) {
-    const unsigned long long oc = __shfl_up(sc, o, MS_WAVE), om = __shfl_up(sm, o, MS_WAVE);
-    if (lane >= o) { sc += oc; sm += om; }
-  }
-  if (t == 0) { found.bin = -1; lowest = bins; }
-  __syncthreads();
-  if (lane == MS_WAVE - 1) { wave_c[wave] = sc; wave_m[wave] = sm; }
-  __syncthreads();
-  unsigned long long before_c = 0, before_m = 0;
-  for (int w = 0; w < wave; ++w) { before_c += wave_c[w]; before_m += wave_m[w]; }
-  unsigned long long run_c = before_c + sc - (c[0] + c[1]), run_m = before_m + sm - (m[0] + m[1]);   // above bin hi
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if (hi - j < 0) break;
-    const unsigned long long upto = (by_mass ? run_m + m[j] : run_c + c[j]), above = by_mass ? run_m : run_c;
-    if (above < need && upto >= need) found = Found{hi - j, run_c, run_m, c[j], m[j]};   // one thread at most
-    if (c[j]) atomicMin(&lowest, hi - j);
-    run_c += c[j]; run_m += m[j];
-  }
-  __syncthreads();
-  if (found.bin < 0 && t == 0) {   // fewer tokens (or less mass) than asked for: everything is kept
-    const int b = lowest < bins ? lowest : 0;
-    unsigned long long tc = 0, tm = 0;
-    for (int w = 0; w < THREADS / MS_WAVE; ++w) { tc += wave_c[w]; tm += wave_m[w]; }
-    found = Found{b, tc - count[b], tm - mass[b], count[b], mass[b]};
-  }
-  __syncthreads();
-  const Found f = found;
-  __syncthreads();
-  return f;
 }
 
 __device__ __forceinline__ void chunk_range(int V, int n_chunks, int c, int* begin, int* end) {
@@ -431,45 +322,6 @@ sample_draw_kernel(const float* __restrict__ logits, size_t ld, int V, const flo
   if (threadIdx.x == 0) out[r] = top.i == 0x7fffffff ? 0 : top.i;
 }
 
-// The distribution the draw is made from: mass / total of what is kept, 0 elsewhere.  A row without temperature, or without
-// any mass (NaN or -inf only), has a one where the greedy choice stands.
-__global__ void __launch_bounds__(THREADS)
-probabilities_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
-                     const RowWork* __restrict__ work, int n_chunks, float* __restrict__ out, size_t out_ld) {
-  __shared__ MaxIdx red_mi[THREADS / MS_WAVE];
-  const int r = blockIdx.y, c = blockIdx.x;
-  const RowWork& w = work[r];
-  const float* row = logits + (size_t)r * ld;
-  float* to = out + (size_t)r * out_ld;
-  int begin, end;
-  chunk_range(V, n_chunks, c, &begin, &end);
-  const float T = temperature[r];
-  int one = -1;
-  unsigned long long total = 0;
-  if (!(T > 0.f)) {
-    MaxIdx top = {-INFINITY, 0x7fffffff};
-    for (int k = 0; k < n_chunks; ++k) top = better(top, MaxIdx{__uint_as_float(w.chunk_max[k]), (int)w.chunk_mass[k]});
-    one = top.i == 0x7fffffff ? 0 : top.i;
-  } else {
-    for (int k = 0; k < n_chunks; ++k) total += w.chunk_mass[k];
-    if (total == 0) {
-      const MaxIdx top = block_argmax(row, 0, V, red_mi);
-      one = top.i == 0x7fffffff ? 0 : top.i;
-    }
-  }
-  if (one >= 0) {
-    for (int i = begin + threadIdx.x; i < end; i += THREADS) to[i] = i == one ? 1.f : 0.f;
-    return;
-  }
-  const unsigned floor_key = w.floor_key;
-  const float inv_t = 1.0f / T, zmax = key_value(row_max_key(w, n_chunks));
-  const float inv = (float)((double)(1ull << FIX_PLACES) / (double)total);
-  for_share(row, begin, end, [&](int i, float v) {
-    const float s = v * inv_t;
-    to[i] = s == s && order_key(s) >= floor_key ? expf(s - zmax) * inv : 0.f;
-  });
-}
-
 // First maximum of a row in two stages, so that a few rows still use the whole chip: stage 1 finds the best
 // of each of n_chunks slices of the row, stage 2 the best of those (larger value, then smaller index).
 __global__ void __launch_bounds__(256)
@@ -584,19 +436,25 @@ extern "C" int ms_argmax_static(const float* logits, long long ld, int n_rows, i
 // Bytes of workspace ms_sample needs for n_rows rows (any contents: the first kernel makes it ready).
 extern "C" long long ms_sample_workspace_bytes(int n_rows) { return (long long)sizeof(RowWork) * (n_rows > 0 ? n_rows : 0); }
 
-// About one block for every CU, but 8 to 24 to a row: every block of a row adds its histogram to the row's with
-// atomics on the same few bins, and reads the histogram of the level before whole, so more blocks to a row cost
-// more than they spread (8 rows of 151,936: 113 us with 64 blocks a row, 71 with 24; 64 rows: 141 us with 8,
-// 179 with 4, 182 with 16).
-static int sample_chunks(int n_rows, int vocab) {
+// One token per row.  Rows with temperature <= 0 (or a null temperature) take the first maximum.  use_top_k /
+// use_top_p: 0 if no row has a top_k in (0, vocab) / a top_p below 1 (their kernels are then left out; when in
+// doubt pass 1).  workspace: ms_sample_workspace_bytes(n_rows) bytes, 8-byte aligned.
+extern "C" int ms_sample(const float* logits, long long ld, int n_rows, int vocab, const float* temperature,
+                         const int* top_k, const float* top_p, const unsigned long long* seeds,
+                         const int* draw_index, int* out, void* workspace, int use_top_k, int use_top_p,
+                         hipStream_t stream) {
+  if (n_rows <= 0) return MS_OK;
+  if (vocab <= 0 || ld < vocab || n_rows > 65535) return MS_BAD_ARG;
+  if (temperature == nullptr) return MS_BAD_ARG;      // all rows greedy: ms_argmax is the entry for that
+  if (workspace == nullptr || ((uintptr_t)workspace % 8)) return MS_BAD_ARG;
+  RowWork* work = (RowWork*)workspace;
+  // About one block for every CU, but 8 to 24 to a row: every block of a row adds its histogram to the row's with
+  // atomics on the same few bins, and reads the histogram of the level before whole, so more blocks to a row cost
+  // more than they spread (8 rows of 151,936: 113 us with 64 blocks a row, 71 with 24; 64 rows: 141 us with 8,
+  // 179 with 4, 182 with 16).
   int n_chunks = ms_compute_units() / n_rows;
   n_chunks = std::max(8, std::min(n_chunks, 24));
-  return std::max(1, std::min(std::min(n_chunks, MAX_CHUNKS), (vocab + 2047) / 2048));
-}
-
-// The kernels up to every chunk's kept mass.
-static void sample_thresholds(const float* logits, long long ld, int n_rows, int vocab, const float* temperature, const int* top_k,
-                              const float* top_p, RowWork* work, int n_chunks, int use_top_k, int use_top_p, hipStream_t stream) {
+  n_chunks = std::max(1, std::min(std::min(n_chunks, MAX_CHUNKS), (vocab + 2047) / 2048));
   const dim3 grid(n_chunks, n_rows), block(THREADS);
   if (top_k == nullptr) use_top_k = 0;
   if (top_p == nullptr) use_top_p = 0;
@@ -613,36 +471,6 @@ static void sample_thresholds(const float* logits, long long ld, int n_rows, int
       sample_level_kernel<3><<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks, 3);
   }
   sample_chunk_mass_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, use_top_p ? top_p : nullptr, work, n_chunks, thresholds);
-}
-
-// One token per row.  Rows with temperature <= 0 (or a null temperature) take the first maximum.  use_top_k /
-// use_top_p: 0 if no row has a top_k in (0, vocab) / a top_p below 1 (their kernels are then left out; when in
-// doubt pass 1).  workspace: ms_sample_workspace_bytes(n_rows) bytes, 8-byte aligned.
-extern "C" int ms_sample(const float* logits, long long ld, int n_rows, int vocab, const float* temperature,
-                         const int* top_k, const float* top_p, const unsigned long long* seeds,
-                         const int* draw_index, int* out, void* workspace, int use_top_k, int use_top_p,
-                         hipStream_t stream) {
-  if (n_rows <= 0) return MS_OK;
-  if (vocab <= 0 || ld < vocab || n_rows > 65535) return MS_BAD_ARG;
-  if (temperature == nullptr) return MS_BAD_ARG;      // all rows greedy: ms_argmax is the entry for that
-  if (workspace == nullptr || ((uintptr_t)workspace % 8)) return MS_BAD_ARG;
-  RowWork* work = (RowWork*)workspace;
-  const int n_chunks = sample_chunks(n_rows, vocab);
-  sample_thresholds(logits, ld, n_rows, vocab, temperature, top_k, top_p, work, n_chunks, use_top_k, use_top_p, stream);
-  sample_draw_kernel<<<dim3(n_rows), dim3(THREADS), 0, stream>>>(logits, (size_t)ld, vocab, temperature, seeds, draw_index, work, n_chunks, out);
-  return ms_launch_status();
-}
-
-// out[r, :] = the distribution ms_sample would draw row r's token from; arguments as there.
-extern "C" int ms_probabilities(const float* logits, long long ld, int n_rows, int vocab, const float* temperature,
-                                const int* top_k, const float* top_p, float* out, long long out_ld, void* workspace,
-                                int use_top_k, int use_top_p, hipStream_t stream) {
-  if (n_rows <= 0) return MS_OK;
-  if (vocab <= 0 || ld < vocab || out_ld < vocab || n_rows > 65535 || temperature == nullptr) return MS_BAD_ARG;
-  if (workspace == nullptr || ((uintptr_t)workspace % 8)) return MS_BAD_ARG;
-  RowWork* work = (RowWork*)workspace;
-  const int n_chunks = sample_chunks(n_rows, vocab);
-  sample_thresholds(logits, ld, n_rows, vocab, temperature, top_k, top_p, work, n_chunks, use_top_k, use_top_p, stream);
-  probabilities_kernel<<<dim3(n_chunks, n_rows), dim3(THREADS), 0, stream>>>(logits, (size_t)ld, vocab, temperature, work, n_chunks, out, (size_t)out_ld);
+  sample_draw_kernel<<<dim3(n_rows), block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, seeds, draw_index, work, n_chunks, out);
   return ms_launch_status();
 }

@@ -118,6 +118,7 @@ _SIGNATURES = {
     "ms_sample": [_c_ptr, _c_ll, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
                   _c_ptr],
     "ms_sample_workspace_bytes": [_c_int],
+    "ms_probabilities_workspace_bytes": [_c_int],
     "ms_probabilities": [_c_ptr, _c_ll, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_int, _c_int, _c_ptr],
     "ms_tree_attention_generic": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                   _c_int, _c_ptr, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int,
@@ -204,7 +205,7 @@ _SIGNATURES = {
                        _c_int, _c_int, _c_ptr],
 }
 
-_RETURNS_LL = ("ms_sample_workspace_bytes", "ms_float_layers_work")     # the others return an int
+_RETURNS_LL = ("ms_sample_workspace_bytes", "ms_probabilities_workspace_bytes", "ms_float_layers_work")     # the others return an int
 
 _fn = {}
 
@@ -1484,12 +1485,23 @@ def paged_attention(q: torch.Tensor, kv, ctx, out: torch.Tensor, num_heads: int,
 
 
 # ------------------------------------------------------------------------------------------------ trees of drafted tokens
+def _device() -> int:
+    return _raw_device() if _raw_device is not None else torch.cuda.current_device()
+
+
 def _here(*tensors) -> None:
     """Work goes to the current device's current stream: tensors of another device are refused."""
-    device = torch.cuda.current_device()
+    device = _device()
     for t in tensors:
         if t is not None and t.get_device() != device:
             raise ValueError(f"a tensor is on cuda:{t.get_device()}, the current device is cuda:{device}")
+
+
+def _need(t: torch.Tensor, name: str, dtype, shape: tuple, device: int) -> None:
+    """``_check`` and ``_here`` of one tensor; what fits takes a third of their time (ten tensors 3 us in place of 10)."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous()):
+        _check(t, name, dtype, shape)
+        _here(t)
 
 
 def probabilities(logits: torch.Tensor, out: torch.Tensor, temperature: Optional[torch.Tensor] = None,
@@ -1499,11 +1511,11 @@ def probabilities(logits: torch.Tensor, out: torch.Tensor, temperature: Optional
     tokens that top-k and top-p keep, 0 elsewhere; with ``temperature`` <= 0 (or without one) a one at the first maximum.
     NaN logits get 0; a row without any mass (NaN or -inf only) has its one where the greedy choice stands.  float32
     [M, V] both, ``out`` another tensor than ``logits``; the other arguments as for ``sample``."""
-    _check(logits, "logits", torch.float32)
-    if logits.dim() != 2:
-        raise ValueError(f"logits must be [rows, vocabulary], got {list(logits.shape)}")
+    device = _device()
+    _check(logits, "logits", torch.float32, (None, None))
+    _here(logits)
     M, V = logits.shape
-    _check(out, "out", torch.float32, (M, V))
+    _need(out, "out", torch.float32, (M, V), device)
     if M > 65535:
         raise ValueError("at most 65,535 rows to a call")
     if M == 0 or V == 0:
@@ -1512,22 +1524,13 @@ def probabilities(logits: torch.Tensor, out: torch.Tensor, temperature: Optional
         raise ValueError("out must not share memory with logits")
     for t, name, dt in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32)):
         if t is not None:
-            _check(t, name, dt, (M,))
-    _here(logits, out, temperature, top_k, top_p)
+            _need(t, name, dt, (M,), device)
     if temperature is None:
         temperature = torch.zeros(M, dtype=torch.float32, device=logits.device)
-    work = torch.empty(int(_get("ms_sample_workspace_bytes")(M)), dtype=torch.uint8, device=logits.device)
+    work = torch.empty(int(_get("ms_probabilities_workspace_bytes")(M)), dtype=torch.uint8, device=logits.device)
     _call("ms_probabilities", logits.data_ptr(), V, M, V, temperature.data_ptr(), _ptr(top_k), _ptr(top_p), out.data_ptr(), V,
           work.data_ptr(), int(use_top_k and top_k is not None), int(use_top_p and top_p is not None), _stream())
     return out
-
-
-def _tree_words(tree: torch.Tensor, n_tokens: int, max_q_len: int) -> int:
-    """The words a token has of its mask."""
-    _check(tree, "tree", torch.int32, (n_tokens, None))
-    if tree.shape[1] * 32 < max_q_len or tree.shape[1] == 0:
-        raise ValueError(f"tree has {tree.shape[1]} words of 32 bits a token for trees of up to {max_q_len} tokens")
-    return tree.shape[1]
 
 
 def tree_attention_generic(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -1536,18 +1539,15 @@ def tree_attention_generic(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
                            table_rows: Optional[torch.Tensor] = None, n_live_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``tree_attention`` on the vector ALUs: float32 or bfloat16, keys and values of any size up to 256, pages of any size.
     Tensors as for ``paged_attention_generic``, q_start int32 [R + 1], context_lens int32 [R]."""
-    _check(k_pages, "k_pages")
+    if k_pages.dim() != 4 or v_pages.dim() != 4:
+        raise ValueError("pages must be [pages, heads, page size, width]")
     P, nkv, page_size, d = k_pages.shape
-    _check(v_pages, "v_pages", k_pages.dtype, (P, nkv, None, None))
     dv = v_pages.shape[2] if v_transposed else v_pages.shape[3]
-    _check(v_pages, "v_pages", k_pages.dtype, _v_shape(k_pages, v_transposed, dv))
-    q_stride = _tree_step(q, k_pages, block_table, q_start, context_lens, table_rows, out, num_heads, nkv, d, dv, max_q_len)
+    q_stride, words = _tree_step(q, k_pages, v_pages, _v_shape(k_pages, v_transposed, dv), block_table, token_req, q_start, context_lens, tree,
+                                 table_rows, out, num_heads, dv, max_q_len)
     N = q.shape[0]
-    words = _tree_words(tree, N, max_q_len)
-    _check(token_req, "token_req", torch.int32, (N,))
     if n_live_tokens is not None:
-        _check(n_live_tokens, "n_live_tokens", torch.int32, (1,))
-    _here(q, k_pages, v_pages, block_table, table_rows, token_req, q_start, context_lens, n_live_tokens, tree, out)
+        _need(n_live_tokens, "n_live_tokens", torch.int32, (1,), _device())
     _call("ms_tree_attention_generic", q.data_ptr(), q_stride, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
           block_table.shape[1], _ptr(table_rows), token_req.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(),
           _ptr(n_live_tokens), tree.data_ptr(), words, out.data_ptr(), num_heads * dv, N, num_heads, nkv, d, dv, page_size,
@@ -1562,14 +1562,12 @@ def tree_attention_mfma(q: torch.Tensor, k_pages: torch.Tensor, vt_pages: torch.
     """``tree_attention`` on the matrix cores: bfloat16, heads of 32, 64 or 128 entries, value pages of that size transposed,
     pages of a multiple of 16 tokens, a positive scale.  ``max_q_len`` and ``max_context_len`` are upper bounds; tokens from
     q_start[R] on belong to no request, a request may have no token."""
-    _check(k_pages, "k_pages", torch.bfloat16)
+    if k_pages.dtype != torch.bfloat16 or k_pages.dim() != 4:
+        raise TypeError("pages must be bfloat16, [pages, heads, page size, width]")
     P, nkv, page_size, d = k_pages.shape
-    _check(vt_pages, "vt_pages", torch.bfloat16, (P, nkv, d, page_size))
-    q_stride = _tree_step(q, k_pages, block_table, q_start, context_lens, table_rows, out, num_heads, nkv, d, d, max_q_len)
-    N, R = q.shape[0], context_lens.numel()
-    words = _tree_words(tree, N, max_q_len)
-    _check(token_req, "token_req", torch.int32, (N,))
-    _here(q, k_pages, vt_pages, block_table, table_rows, token_req, q_start, context_lens, tree, out)
+    q_stride, words = _tree_step(q, k_pages, vt_pages, (P, nkv, d, page_size), block_table, token_req, q_start, context_lens, tree, table_rows, out,
+                                 num_heads, d, max_q_len)
+    N, R = q.shape[0], context_lens.shape[0]
     if N == 0 or R == 0:
         return out
     plan = _get("ms_tree_attention_mfma_plan")(R, N, max_q_len, max_context_len, num_heads, nkv, d, page_size)
@@ -1586,26 +1584,38 @@ def tree_attention_mfma(q: torch.Tensor, k_pages: torch.Tensor, vt_pages: torch.
     return out
 
 
-def _tree_step(q, k_pages, block_table, q_start, context_lens, table_rows, out, num_heads, nkv, d, dv, max_q_len) -> int:
-    """Checks what the kernels of ``tree_attention`` have in common; the stride of q's rows."""
-    stride = _rows2d(q, "q", k_pages.dtype)
+def _tree_step(q, k_pages, v_pages, v_shape, block_table, token_req, q_start, context_lens, tree, table_rows, out, num_heads, dv, max_q_len):
+    """Checks what the kernels of ``tree_attention`` have in common; the stride of q's rows and the words of a token's mask."""
+    device, (P, nkv, page_size, d) = _device(), k_pages.shape
+    dtype, i32 = k_pages.dtype, torch.int32
+    _code(dtype)
+    _need(k_pages, "k_pages", dtype, (P, nkv, page_size, d), device)
+    _need(v_pages, "v_pages", dtype, v_shape, device)
+    stride = _rows2d(q, "q", dtype)
+    _here(q)
     N = q.shape[0]
     if q.shape[1] < num_heads * d:
         raise ValueError(f"q must be [N, >= {num_heads * d}], got {list(q.shape)}")
-    if num_heads <= 0 or num_heads % nkv:
+    if num_heads <= 0 or nkv <= 0 or num_heads % nkv:
         raise ValueError(f"{num_heads} query heads cannot share {nkv} key/value heads")
-    _check(out, "out", k_pages.dtype, (N, num_heads * dv))
-    _check(block_table, "block_table", torch.int32, (None, None))
-    _check(context_lens, "context_lens", torch.int32, (None,))
-    R = context_lens.numel()
-    _check(q_start, "q_start", torch.int32, (R + 1,))
+    _need(out, "out", dtype, (N, num_heads * dv), device)
+    if block_table.dim() != 2 or context_lens.dim() != 1 or tree.dim() != 2:
+        raise ValueError("block_table must be [rows, pages], context_lens [requests], tree [tokens, words]")
+    R, words = context_lens.shape[0], tree.shape[1]
+    _need(block_table, "block_table", i32, tuple(block_table.shape), device)
+    _need(context_lens, "context_lens", i32, (R,), device)
+    _need(q_start, "q_start", i32, (R + 1,), device)
+    _need(token_req, "token_req", i32, (N,), device)
+    _need(tree, "tree", i32, (N, words), device)
     if table_rows is not None:
-        _check(table_rows, "table_rows", torch.int32, (R,))
+        _need(table_rows, "table_rows", i32, (R,), device)
     elif block_table.shape[0] < R:
         raise ValueError(f"the block table has {block_table.shape[0]} rows for {R} requests")
     if max_q_len < 1:
         raise ValueError(f"max_q_len {max_q_len}: a tree has at least one token")
-    return stride
+    if words == 0 or words * 32 < max_q_len:
+        raise ValueError(f"tree has {words} words of 32 bits a token for trees of up to {max_q_len} tokens")
+    return stride, words
 
 
 def tree_attention(q: torch.Tensor, kv, ctx, tree: torch.Tensor, out: torch.Tensor, num_heads: int, scale: float) -> torch.Tensor:
@@ -1639,25 +1649,26 @@ def verify_drafts(p: torch.Tensor, q: Optional[torch.Tensor], token_ids: torch.T
 
     nodes[r] int32 [R, depth]: the accepted path's rows, 0 first, then -1; a path that fills it ends there.  counts[r]: its
     length.  out[r]: the token drawn behind it.  A request without rows gets -1, 0 and -1."""
-    _check(p, "p", torch.float32, (None, None))
+    device, f32, i32 = _device(), torch.float32, torch.int32
+    _check(p, "p", f32, (None, None))
+    _here(p)
     N, V = p.shape
     if V == 0:
         raise ValueError("p has no vocabulary")
     if q is not None:
-        _check(q, "q", torch.float32, (N, V))
-    _check(token_ids, "token_ids", torch.int32, (N,))
-    _check(parents, "parents", torch.int32, (N,))
-    _check(uniforms, "uniforms", torch.float32, (N,))
-    _check(q_start, "q_start", torch.int32, (None,))
+        _need(q, "q", f32, (N, V), device)
+    _need(token_ids, "token_ids", i32, (N,), device)
+    _need(parents, "parents", i32, (N,), device)
+    _need(uniforms, "uniforms", f32, (N,), device)
     R = q_start.numel() - 1
     if R < 0 or R > 65535:
         raise ValueError("q_start has one number more than there are requests, at most 65,536")
-    _check(nodes, "nodes", torch.int32, (R, None))
-    if nodes.shape[1] < 1:
-        raise ValueError("nodes must have room for the root")
-    _check(counts, "counts", torch.int32, (R,))
-    _check(out, "out", torch.int32, (R,))
-    _here(p, q, token_ids, parents, q_start, uniforms, nodes, counts, out)
+    _need(q_start, "q_start", i32, (R + 1,), device)
+    if nodes.dim() != 2 or nodes.shape[1] < 1:
+        raise ValueError("nodes must be [requests, depth], with room for the root")
+    _need(nodes, "nodes", i32, (R, nodes.shape[1]), device)
+    _need(counts, "counts", i32, (R,), device)
+    _need(out, "out", i32, (R,), device)
     _call("ms_verify_drafts", p.data_ptr(), _ptr(q), N, V, token_ids.data_ptr(), parents.data_ptr(), q_start.data_ptr(),
           uniforms.data_ptr(), R, nodes.data_ptr(), nodes.shape[1], counts.data_ptr(), out.data_ptr(), _stream())
     return out
@@ -1676,18 +1687,21 @@ def keep_tokens(pages, transposed, block_table: torch.Tensor, first: torch.Tenso
     most = _get("ms_keep_tokens_max")()
     if len(pages) > most:
         raise ValueError(f"at most {most} page tensors to a call")
-    _check(nodes, "nodes", torch.int32, (None, None))
+    device, i32 = _device(), torch.int32
+    if nodes.dim() != 2 or block_table.dim() != 2:
+        raise ValueError("nodes must be [requests, depth], block_table [rows, pages]")
     R, depth = nodes.shape
-    _check(first, "first", torch.int32, (R,))
-    _check(counts, "counts", torch.int32, (R,))
-    _check(block_table, "block_table", torch.int32, (None, None))
+    _need(nodes, "nodes", i32, (R, depth), device)
+    _need(first, "first", i32, (R,), device)
+    _need(counts, "counts", i32, (R,), device)
+    _need(block_table, "block_table", i32, tuple(block_table.shape), device)
     if table_rows is not None:
-        _check(table_rows, "table_rows", torch.int32, (R,))
+        _need(table_rows, "table_rows", i32, (R,), device)
     elif block_table.shape[0] < R:
         raise ValueError(f"the block table has {block_table.shape[0]} rows for {R} requests")
     sizes = []
     for t, flip in zip(pages, transposed):
-        _check(t, "pages", pages[0].dtype)
+        _need(t, "pages", pages[0].dtype, tuple(t.shape), device)
         if t.dim() not in (4, 5):
             raise ValueError(f"pages must be [layers, pages, heads, page size, width] or without the layers, got {list(t.shape)}")
         L, P, heads, a, b = t.shape if t.dim() == 5 else (1, *t.shape)
@@ -1700,7 +1714,6 @@ def keep_tokens(pages, transposed, block_table: torch.Tensor, first: torch.Tenso
         return
     if R > 65535:
         raise ValueError("at most 65,535 requests to a call")
-    _here(*pages, block_table, first, nodes, counts, table_rows)
     keep, ptrs = _pointer_array(pages)
     n = len(pages)
     ints = [(_c_int * n)(*v) for v in ([s[3] for s in sizes], [s[4] for s in sizes], [int(bool(f)) for f in transposed])]

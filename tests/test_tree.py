@@ -734,6 +734,7 @@ def host(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "is_cuda", True, raising=False)
     launched = []
     monkeypatch.setattr(ops, "_here", lambda *a: None)
+    monkeypatch.setattr(ops, "_device", lambda: -1)
     monkeypatch.setattr(ops, "_call", lambda name, *a: launched.append(name))
     monkeypatch.setattr(ops, "_stream", lambda: 0)
     monkeypatch.setattr(ops, "_get", lambda name: (lambda *a: {"ms_keep_tokens_max": 16}.get(name, 64)))
