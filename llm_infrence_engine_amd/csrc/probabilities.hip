@@ -19,6 +19,7 @@
 #include "sampling.h"
 #include "api.h"
 #include <algorithm>
+#include <type_traits>
 
 // A scaled logit is rounded to a float before anything else is done with it: its key, its mass and its probability are those of one
 // number, wherever they are worked out (a product joined with the subtraction of the maximum is another one).
@@ -77,40 +78,64 @@ __device__ __forceinline__ void quad_range(const float* row, int V, int n_chunks
   *end = min(quads, *begin + len);
 }
 
-// f(i, v): the values i .. i + 3 of this thread's quads begin .. end - 1 (places outside the row: NaN), four quads under way at a
-// time and none behind a condition; the quads at a row's ends, which may lie in part outside of it, value by value.
+// f(i, v): the values i .. i + 3 of this thread's quads begin .. end - 1 (places outside the row: NaN).  Four quads are under way at
+// a time, none behind a condition; the quads at a row's ends, which may lie in part outside of it, come last, value by value.
 template <typename F>
 __device__ __forceinline__ void for_quads(const float* __restrict__ row, int V, int begin, int end, F f) {
   constexpr int AT_ONCE = 4;
-  const int lead = lead_of(row), first = lead ? 1 : 0, last = (lead + V) / 4 - 1;      // the whole quads
+  const int lead = lead_of(row), first = max(begin, lead ? 1 : 0), until = min(end, (lead + V) / 4);      // the whole quads
   const float* base = row - lead;
-  for (int q0 = begin + threadIdx.x; q0 < end; q0 += AT_ONCE * THREADS) {
+  for (int q0 = first + threadIdx.x; q0 < until; q0 += AT_ONCE * THREADS) {
     float4 v[AT_ONCE];
-    if (first <= last) {
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) v[j] = *reinterpret_cast<const float4*>(base + 4 * (size_t)min(max(q0 + j * THREADS, first), last));
+    for (int j = 0; j < AT_ONCE; ++j) v[j] = *reinterpret_cast<const float4*>(base + 4 * (size_t)min(q0 + j * THREADS, until - 1));
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+      if (q0 + j * THREADS < until) f(4 * (q0 + j * THREADS) - lead, v[j]);
+  }
+  // the first quad of a row that begins inside it, and the last of one that ends inside it
+  const int q = threadIdx.x == 0 ? begin : end - 1;
+  if (threadIdx.x < 2 && begin < end && (q < first || q >= until) && (threadIdx.x == 0 || end - 1 != begin)) {
+    float e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = 4 * q - lead + i;
+      e[i] = at >= 0 && at < V ? row[at] : __builtin_nanf("");
     }
-#pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j) {
-      const int q = q0 + j * THREADS;
-      if (q >= end) break;
-      if (q < first || q > last) {
-        float e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = 4 * q - lead + i;
-          e[i] = at >= 0 && at < V ? row[at] : __builtin_nanf("");
-        }
-        v[j] = make_float4(e[0], e[1], e[2], e[3]);
-      }
-      f(4 * q - lead, v[j]);
-    }
+    f(4 * q - lead, make_float4(e[0], e[1], e[2], e[3]));
   }
 }
 template <typename F>
 __device__ __forceinline__ void for_values(const float* __restrict__ row, int V, int begin, int end, F f) {
   for_quads(row, V, begin, end, [&](int, const float4& v) { f(v.x); f(v.y); f(v.z); f(v.w); });
 }
+
+// e^x for x <= 0 by the hardware's exp2, the product with log2(e) in two parts (2 units in the last place); NaN: 0, and below
+// e^-200, which no float holds, 0 too.
+__device__ __forceinline__ float exp_of(float x) {
+  x = fmaxf(x, -200.f);
+  const float t = x * 1.44269502f;
+  const float r = fmaf(x, 1.92596303e-8f, fmaf(x, 1.44269502f, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e * 0.693147181f, r, e);
+}
+
+// e^(s - zmax) cut to 44 binary places, in two words of 20 and 24 (a conversion to 64 bits at once is three times as long).
+struct Mass {
+  unsigned hi, lo;
+  __device__ __forceinline__ explicit Mass(float e) {
+    const float scaled = e * (float)(1u << (FIX_PLACES - 24));
+    hi = (unsigned)scaled;
+    lo = (unsigned)((scaled - (float)hi) * (float)(1u << 24));
+  }
+  __device__ __forceinline__ unsigned long long value() const { return ((unsigned long long)hi << 24) + lo; }
+};
+struct MassSum {
+  unsigned long long hi = 0, lo = 0;
+  __device__ __forceinline__ void add(Mass m) { hi += m.hi; lo += m.lo; }
+  __device__ __forceinline__ unsigned long long value() const { return (hi << 24) + lo; }
+};
+__device__ __forceinline__ unsigned long long mass_of(float s, float zmax) { return Mass(exp_of(s - zmax)).value(); }
 
 __device__ unsigned long long block_sum_u64(unsigned long long v, unsigned long long* red) {
   for (int o = MS_WAVE / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
@@ -122,17 +147,20 @@ __device__ unsigned long long block_sum_u64(unsigned long long v, unsigned long 
   return s;
 }
 
+// Over a row's chunks, a chunk to a lane (a loop over them waits for one after another: 32 of them 10 us).
 __device__ __forceinline__ unsigned largest_key(const RowWork& w, int n_chunks) {
-  unsigned best = 0;
-  for (int c = 0; c < n_chunks; ++c) best = max(best, w.chunk_max[c]);
-  return best;
+  const int lane = threadIdx.x & (MS_WAVE - 1);
+  unsigned best = lane < n_chunks ? w.chunk_max[lane] : 0u;
+  for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) best = max(best, (unsigned)__shfl_xor((int)best, o, MS_WAVE));
+  return __builtin_amdgcn_readfirstlane(best);
+}
+__device__ __forceinline__ unsigned long long sum_of(const unsigned long long* chunks, int n_chunks) {
+  const int lane = threadIdx.x & (MS_WAVE - 1);
+  unsigned long long v = lane < n_chunks ? chunks[lane] : 0ull;
+  for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
+  return __shfl(v, 0, MS_WAVE);
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
-
-__device__ __forceinline__ int bin_of(float s, float zmax) {      // BINS: beyond them, or NaN
-  const float x = (zmax - s) * BINS_A_UNIT;
-  return x < (float)BINS ? (int)x : BINS;
-}
 
 // ---- 1
 __global__ void __launch_bounds__(THREADS)
@@ -193,8 +221,7 @@ __global__ void __launch_bounds__(THREADS)
 probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
                              const int* __restrict__ top_k, const float* __restrict__ top_p, RowWork* __restrict__ work, int n_chunks) {
   __shared__ unsigned long long red[WAVES];
-  __shared__ unsigned keys[MAX_CHUNKS * WAVES * 4];
-  __shared__ unsigned bound_sm;
+  __shared__ float hist[BINS];
   const int r = blockIdx.y, c = blockIdx.x;
   RowWork& w = work[r];
   const RowPlan a = plan_of(temperature, top_k, top_p, r, V, n_chunks);
@@ -213,21 +240,39 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
   }
   if (a.k) {
     if (!a.groups) return;
-    const int n = n_chunks * WAVES * a.groups;
-    for (int i = threadIdx.x; i < n; i += THREADS) keys[i] = w.groups[i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += THREADS) {      // the k-th largest of them
-      const unsigned mine = keys[i];
-      int above = 0, equal = 0;
-      for (int j = 0; j < n; j += 4) {                    // (n is a multiple of 16)
-        const uint4 o = *reinterpret_cast<const uint4*>(&keys[j]);
-        above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
-        equal += (o.x == mine) + (o.y == mine) + (o.z == mine) + (o.w == mine);
+    // the k-th largest of the group maxima, bit by bit; every wave does it for itself, N keys to a lane
+    const int n = n_chunks * WAVES * a.groups, lane = threadIdx.x & (MS_WAVE - 1);
+    auto kth = [&](auto size) __attribute__((always_inline)) {
+      constexpr int N = decltype(size)::value;
+      unsigned key[N], most = 0u, least = 0xffffffffu;
+#pragma unroll
+      for (int i = 0; i < N; ++i) key[i] = w.groups[min(lane + i * MS_WAVE, n - 1)];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (lane + i * MS_WAVE >= n) key[i] = 0u;         // (the bound of k <= n keys is no smaller for them)
+        most = max(most, key[i]);
+        least = min(least, key[i]);
       }
-      if (above < a.k && a.k <= above + equal) bound_sm = mine;      // (all who find it find the same)
-    }
-    __syncthreads();
-    const unsigned bound = bound_sm;
+      for (int o = MS_WAVE / 2; o > 0; o >>= 1) {
+        most = max(most, (unsigned)__shfl_xor((int)most, o, MS_WAVE));
+        least = min(least, (unsigned)__shfl_xor((int)least, o, MS_WAVE));
+      }
+      most = __builtin_amdgcn_readfirstlane(most);
+      least = __builtin_amdgcn_readfirstlane(least);
+      if (most == least) return most;
+      int bit = 31 - __builtin_clz(most ^ least);         // above it all keys are alike
+      unsigned prefix = most & ~(0xffffffffu >> (31 - bit));
+      for (; bit >= 0; --bit) {
+        const unsigned with = prefix | (1u << bit);
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) count += __builtin_popcountll(__ballot(key[i] >= with));
+        if (count >= a.k) prefix = with;
+      }
+      return prefix;
+    };
+    const unsigned bound = n <= 4 * MS_WAVE ? kth(std::integral_constant<int, 4>{}) : n <= 8 * MS_WAVE ? kth(std::integral_constant<int, 8>{})
+                                                                                    : kth(std::integral_constant<int, MAX_CHUNKS * WAVES * 4 / MS_WAVE>{});
     unsigned ties = 0;
     for_values(row, V, begin, end, [&](float v) {
       const float s = v * a.inv_t;
@@ -246,31 +291,23 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
     }
     return;
   }
-  unsigned long long mine = 0;
+  MassSum mine;
   if (!a.use_p) {
-    for_values(row, V, begin, end, [&](float v) {
-      const float s = v * a.inv_t;
-      if (s == s) mine += fixed_mass(s, zmax);
-    });
+    for_values(row, V, begin, end, [&](float v) { mine.add(Mass(exp_of(v * a.inv_t - zmax))); });
   } else {
-    float* hist = reinterpret_cast<float*>(keys);      // BINS of them
-    static_assert(sizeof(keys) >= BINS * sizeof(float), "the histogram fits");
     for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0.f;
     __syncthreads();
     for_values(row, V, begin, end, [&](float v) {
-      const float s = v * a.inv_t;
-      if (!(s == s)) return;
-      const float e = expf(s - zmax);
-      mine += (unsigned long long)(e * (float)(1ull << FIX_PLACES));      // (fixed_mass)
-      const int bin = bin_of(s, zmax);
-      if (bin < BINS) unsafeAtomicAdd(&hist[bin], e);
+      const float s = v * a.inv_t, e = exp_of(s - zmax), x = (zmax - s) * BINS_A_UNIT;
+      mine.add(Mass(e));
+      if (x < (float)BINS) unsafeAtomicAdd(&hist[(int)x], e);
     });
     __syncthreads();
     for (int i = threadIdx.x; i < BINS; i += THREADS)
       if (hist[i] != 0.f) unsafeAtomicAdd(&w.hist[i], hist[i]);
   }
-  mine = block_sum_u64(mine, red);
-  if (threadIdx.x == 0) w.chunk_mass[c] = mine;
+  const unsigned long long mass = block_sum_u64(mine.value(), red);
+  if (threadIdx.x == 0) w.chunk_mass[c] = mass;
 }
 
 __device__ __forceinline__ unsigned long long target_of(float p, unsigned long long total) {      // as the sampler has it
@@ -291,8 +328,7 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   if (a.greedy || a.k || !a.use_p || a.all) return;
   const float zmax = key_value(largest_key(w, n_chunks));
   if (!finite(zmax)) return;
-  unsigned long long total = 0;
-  for (int k = 0; k < n_chunks; ++k) total += w.chunk_mass[k];
+  const unsigned long long total = sum_of(w.chunk_mass, n_chunks);
   const float target = (float)((double)target_of(a.p, total) / (double)(1ull << FIX_PLACES));
   // the first bin at which the running mass reaches the target; a thread owns two bins
   const float h0 = w.hist[2 * threadIdx.x], h1 = w.hist[2 * threadIdx.x + 1];
@@ -309,7 +345,8 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   __syncthreads();
   // (sums of floats may fall short of a target that is nearly everything: the last bin that has any would be no surer)
   if (found >= BINS) return;
-  const int lo = found - 1, hi = found + 1;
+  // its bin and the one on either side, as values
+  const float high = zmax - (float)(found - 1) * (1.0f / BINS_A_UNIT), low = zmax - (float)(found + 2) * (1.0f / BINS_A_UNIT);
   if (c == 0 && threadIdx.x == 0) w.bin = found;
   const float* row = logits + (size_t)r * ld;
   int begin, end;
@@ -317,11 +354,9 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   unsigned long long above = 0;
   for_values(row, V, begin, end, [&](float v) {
     const float s = v * a.inv_t;
-    if (!(s == s)) return;
-    const int bin = bin_of(s, zmax);
-    if (bin < lo) {
-      above += fixed_mass(s, zmax);
-    } else if (bin <= hi && bin < BINS) {
+    if (s > high) {
+      above += mass_of(s, zmax);
+    } else if (s >= low) {
       const unsigned at = atomicAdd(&w.n_candidates, 1u);
       if (at < MAX_CANDIDATES) w.candidates[at] = order_key(s);
     }
@@ -349,7 +384,7 @@ __device__ Kept descend(const float* __restrict__ row, int V, const RowPlan& a, 
         const unsigned key = order_key(s);
         const bool in = s == s && key >= least && (level == 1 || (key >> (shift + (level == 2 ? 11 : 10))) == digits);
         const int bin = (int)((key >> shift) & (unsigned)(bins - 1));
-        unsigned long long m = in ? fixed_mass(s, zmax) : 0ull;
+        unsigned long long m = in ? mass_of(s, zmax) : 0ull;
         const unsigned long long who = __ballot(in);
         if (!who) return;
         const int leader = __builtin_ctzll(who);
@@ -409,8 +444,11 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
   const float zmax = a.greedy ? 0.f : key_value(top);
   int one = -1;
   if (a.greedy) {
+    const int lane = threadIdx.x & (MS_WAVE - 1);
     MaxIdx best = {-INFINITY, 0x7fffffff};
-    for (int k = 0; k < n_chunks; ++k) best = better(best, MaxIdx{__uint_as_float(w.chunk_max[k]), (int)w.chunk_mass[k]});
+    if (lane < n_chunks) best = MaxIdx{__uint_as_float(w.chunk_max[lane]), (int)w.chunk_mass[lane]};
+    for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) best = better(best, MaxIdx{__shfl_xor(best.v, o, MS_WAVE), __shfl_xor(best.i, o, MS_WAVE)});
+    best.i = __shfl(best.i, 0, MS_WAVE);
     one = best.i == 0x7fffffff ? 0 : best.i;
   } else if (!finite(zmax)) {
     const MaxIdx best = block_argmax(row, 0, V, red_mi);
@@ -427,7 +465,7 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
 
   Kept kept = {0u, 0ull};
   if (!a.k && !a.use_p) {
-    for (int k = 0; k < n_chunks; ++k) kept.mass += w.chunk_mass[k];
+    kept.mass = sum_of(w.chunk_mass, n_chunks);
   } else {
     const int n = (int)w.n_candidates;
     bool known = n <= MAX_CANDIDATES && (a.all || (a.k ? a.groups > 0 : w.bin >= 0));
@@ -435,17 +473,16 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
       // a thread to a candidate; values equal to the bound are one more, as often as they were counted
       const bool tied = a.k && !a.all;
       const unsigned ties = tied ? w.n_ties : 0u;
-      const unsigned long long tie_mass = tied ? fixed_mass(key_value(w.bound), zmax) : 0ull;
+      const unsigned long long tie_mass = tied ? mass_of(key_value(w.bound), zmax) : 0ull;
       unsigned mine = 0u;
       unsigned long long mass = 0ull, above_all = 0ull;
       if ((int)threadIdx.x < n) {
         mine = w.candidates[threadIdx.x];
-        mass = fixed_mass(key_value(mine), zmax);
+        mass = mass_of(key_value(mine), zmax);
         keys[threadIdx.x] = mine;
         masses[threadIdx.x] = mass;
       }
-      if (!a.k && !a.all)
-        for (int k = 0; k < n_chunks; ++k) above_all += w.chunk_above[k];
+      if (!a.k && !a.all) above_all = sum_of(w.chunk_above, n_chunks);
       if (threadIdx.x == 0) floor_sm = 0xffffffffu;
       __syncthreads();
       unsigned count = 0;
@@ -460,10 +497,7 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
       bool in = in_k, ties_in = ties_in_k;
       if (a.use_p) {
         unsigned long long whole = total;
-        if (!a.k && !a.all) {
-          whole = 0;
-          for (int k = 0; k < n_chunks; ++k) whole += w.chunk_mass[k];
-        }
+        if (!a.k && !a.all) whole = sum_of(w.chunk_mass, n_chunks);
         const unsigned long long target = target_of(a.p, whole);
         known = above_all < target && total >= target;      // (it falls among the candidates)
         in = in_k && larger < target;
@@ -478,11 +512,11 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
     }
     if (!known) kept = descend(row, V, a, zmax, keys, masses);
   }
-  const float inv = (float)((double)(1ull << FIX_PLACES) / (double)kept.mass);
+  const float inv = (float)((double)(1ull << FIX_PLACES) / (double)kept.mass), floor = kept.floor ? key_value(kept.floor) : -INFINITY;
   for_quads(row, V, begin, end, [&](int i, const float4& v) {
     auto value = [&](float x) {
       const float s = x * a.inv_t;
-      return s == s && order_key(s) >= kept.floor ? expf(s - zmax) * inv : 0.f;
+      return s >= floor ? exp_of(s - zmax) * inv : 0.f;
     };
     store(i, make_float4(value(v.x), value(v.y), value(v.z), value(v.w)));
   });
