@@ -267,7 +267,9 @@ int ms_tree_attention_mfma(const void* q, long long q_stride, const void* k_page
 // [n_requests, depth] (the accepted path, -1 behind it), counts [n_requests], out [n_requests] (the token drawn behind it).
 int ms_verify_drafts(const float* p, const float* q, int n_tokens, int vocab, const int* tokens, const int* parents,
                      const int* q_start, const float* uniforms, int n_requests, int* nodes, int depth, int* counts, int* out,
-                     hipStream_t stream);
+                     void* workspace, hipStream_t stream);
+long long ms_verify_drafts_workspace_bytes(int n_requests);      // of workspace, device memory of any contents
+void ms_verify_drafts_patience(int looks);                       // tests
 
 // pages / heads / widths / transposed: host arrays of n_tensors (at most ms_keep_tokens_max()); pages[i] [layers, num_pages,
 // heads[i], page_size, widths[i]], or [.., widths[i], page_size].  Entry first[r] + nodes[r][i] goes to first[r] + i.

@@ -126,8 +126,10 @@ _SIGNATURES = {
     "ms_tree_attention_mfma_plan": [_c_int] * 8,
     "ms_tree_attention_mfma": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr,
                                _c_ll, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int, _c_ptr],
+    "ms_verify_drafts_workspace_bytes": [_c_int],
+    "ms_verify_drafts_patience": [_c_int],
     "ms_verify_drafts": [_c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr,
-                         _c_ptr],
+                         _c_ptr, _c_ptr],
     "ms_keep_tokens_max": [],
     "ms_keep_tokens": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr,
                        _c_int, _c_ptr, _c_int, _c_int, _c_ptr],
@@ -205,7 +207,7 @@ _SIGNATURES = {
                        _c_int, _c_int, _c_ptr],
 }
 
-_RETURNS_LL = ("ms_sample_workspace_bytes", "ms_probabilities_workspace_bytes", "ms_float_layers_work")     # the others return an int
+_RETURNS_LL = ("ms_sample_workspace_bytes", "ms_probabilities_workspace_bytes", "ms_verify_drafts_workspace_bytes", "ms_float_layers_work")     # the others return an int
 
 _fn = {}
 
@@ -1669,8 +1671,9 @@ def verify_drafts(p: torch.Tensor, q: Optional[torch.Tensor], token_ids: torch.T
     _need(nodes, "nodes", i32, (R, nodes.shape[1]), device)
     _need(counts, "counts", i32, (R,), device)
     _need(out, "out", i32, (R,), device)
+    work = torch.empty(int(_get("ms_verify_drafts_workspace_bytes")(R)), dtype=torch.uint8, device=p.device)
     _call("ms_verify_drafts", p.data_ptr(), _ptr(q), N, V, token_ids.data_ptr(), parents.data_ptr(), q_start.data_ptr(),
-          uniforms.data_ptr(), R, nodes.data_ptr(), nodes.shape[1], counts.data_ptr(), out.data_ptr(), _stream())
+          uniforms.data_ptr(), R, nodes.data_ptr(), nodes.shape[1], counts.data_ptr(), out.data_ptr(), work.data_ptr(), _stream())
     return out
 
 

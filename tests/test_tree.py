@@ -438,6 +438,39 @@ def test_verify_drafts_of_a_large_vocabulary():
 
 
 @gpu
+def test_verify_drafts_without_the_other_blocks():
+    """A leader that does not wait for the other blocks of its request works every sum out itself, to the same result; so does one
+    that waits hardly at all, whatever has come by then."""
+    made = [make_drafts([9, 1, 6, 0, 30], 20001, seed, with_q, near=1.0) for seed, with_q in ((1, True), (2, False), (3, True))]
+    want = [run_verify(*m, 30) for m in made]
+    try:
+        for looks in (-1, 1, 2):
+            ops._get("ms_verify_drafts_patience")(looks)
+            assert [run_verify(*m, 30) for m in made] == want
+    finally:
+        ops._get("ms_verify_drafts_patience")(0)
+    for m in made:
+        check_verify(*m, 30)
+
+
+@gpu
+def test_verify_drafts_of_long_trees_and_many_requests():
+    """More tokens than a block keeps at hand, more children of one token than that, more requests than CUs."""
+    p, q, tokens, parents, starts, u = make_drafts([1500, 3], 40, 3, True, near=1.5, width=2)
+    check_verify(p, q, tokens, parents, starts, u, 64)
+    check_verify(p, None, tokens, parents, starts, u, 64)
+    parents[:1500] = [-1] + [0] * 1499
+    u[:1500] = 1.0 - 2.0 ** -24
+    p[0] = 0.0
+    p[0, 39] = 1e-3
+    p[0, 38] = 1.0 - 1e-3
+    tokens[:1500] = [i % 38 for i in range(1500)]
+    check_verify(p, None, tokens, parents, starts, u, 3)
+    for with_q in (True, False):
+        check_verify(*make_drafts([1 + i % 4 for i in range(400)], 1100, 6, with_q), 4)
+
+
+@gpu
 @pytest.mark.parametrize("with_q", [True, False])
 def test_verify_drafts_edges(with_q):
     """Numbers of zero and next to one, equal distributions, guesses without mass, the same guess twice, guesses that are no
@@ -737,7 +770,7 @@ def host(monkeypatch):
     monkeypatch.setattr(ops, "_device", lambda: -1)
     monkeypatch.setattr(ops, "_call", lambda name, *a: launched.append(name))
     monkeypatch.setattr(ops, "_stream", lambda: 0)
-    monkeypatch.setattr(ops, "_get", lambda name: (lambda *a: {"ms_keep_tokens_max": 16}.get(name, 64)))
+    monkeypatch.setattr(ops, "_get", lambda name: (lambda *a: {"ms_keep_tokens_max": 16}.get(name, 64)))      # (sizes of workspaces)
     return launched
 
 
