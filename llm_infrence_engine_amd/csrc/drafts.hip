@@ -60,6 +60,14 @@ __device__ __forceinline__ double block_sum_double(double v, double* red) {
   return s;
 }
 
+// The chunks' sums added up in a fixed order, a chunk to a lane.
+__device__ __forceinline__ double sum_of(const double* part, int n) {
+  const int lane = threadIdx.x & (MS_WAVE - 1);
+  double v = lane < n ? part[lane] : 0.0;
+  for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
+  return __shfl(v, 0, MS_WAVE);
+}
+
 // What is left of a row of the target: max(0, p - t q); without q p without the tokens of `gone` (of which, with `parents`, those
 // of `parent` count).
 struct Rest {
@@ -293,8 +301,7 @@ verify_drafts_kernel(const float* __restrict__ p, const float* __restrict__ q, i
       if (threadIdx.x == 0) part[k] = sum;
     }
     __syncthreads();
-    S = 0.0;
-    for (int k = 0; k < n_chunks; ++k) S += part[k];
+    S = sum_of(part, n_chunks);
     summed = true;
     __syncthreads();
   }
@@ -303,13 +310,16 @@ verify_drafts_kernel(const float* __restrict__ p, const float* __restrict__ q, i
   // ---- the token behind the path: the chunk in which the mark falls, then the first entry that passes it, 4,096 at a time
   const Rest rest = rest_of(row, order_t);
   const double target = (double)uniforms[t0] * S;
-  int chunk = -1, spare = 0;
-  double run = 0.0;
-  for (int k = 0; k < n_chunks && chunk < 0; ++k) {
-    if (part[k] > 0.0) spare = k;
-    if (run + part[k] > target) chunk = k; else run += part[k];
+  double upto = lane < n_chunks ? part[lane] : 0.0;      // sums over the chunks, one to a lane
+  const double mass = upto;
+  for (int o = 1; o < MAX_CHUNKS; o <<= 1) {
+    const double v = __shfl_up(upto, o, MS_WAVE);
+    if (lane >= o) upto += v;
   }
-  if (chunk < 0) { chunk = spare; run -= part[spare]; }      // (the sum in this order stayed below the mark)
+  const u64 passing_chunks = __ballot(lane < n_chunks && mass > 0.0 && upto > target), some_chunks = __ballot(lane < n_chunks && mass > 0.0);
+  // (a sum in this order may stay below the mark: then the last chunk that has any)
+  const int chunk = passing_chunks ? __builtin_ctzll(passing_chunks) : some_chunks ? 63 - __builtin_clzll(some_chunks) : 0;
+  double run = __shfl(upto - mass, chunk, MS_WAVE);
   if (threadIdx.x == 0) { first_e = V; last_e = -1; }
   __syncthreads();
   const int hi = lo_of(chunk + 1);
@@ -323,28 +333,32 @@ verify_drafts_kernel(const float* __restrict__ p, const float* __restrict__ q, i
       if (e0 + j >= hi) w[j] = 0.0;
       here += w[j];
     }
-    double upto = here;                    // sums over the threads before, in index order
+    double here_upto = here;               // sums over the threads before, in index order
     for (int o = 1; o < MS_WAVE; o <<= 1) {
-      const double v = __shfl_up(upto, o, MS_WAVE);
-      if (lane >= o) upto += v;
+      const double v = __shfl_up(here_upto, o, MS_WAVE);
+      if (lane >= o) here_upto += v;
     }
     __syncthreads();
-    if (lane == MS_WAVE - 1) red[wave] = upto;
+    if (lane == MS_WAVE - 1) red[wave] = here_upto;
     __syncthreads();
     double before = run, all = 0.0;
     for (int k = 0; k < WAVES; ++k) {
       if (k < wave) before += red[k];
       all += red[k];
     }
-    double sum = before + upto - here;
+    double sum = before + here_upto - here;
+    int passes = V, some = -1;             // the thread's first entry that passes the mark, its last that has any weight
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       sum += w[j];
       if (w[j] > 0.0) {
-        if (sum > target) atomicMin(&first_e, e0 + j);
-        atomicMax(&last_e, e0 + j);
+        if (sum > target) passes = min(passes, e0 + j);
+        some = e0 + j;
       }
     }
+    const u64 passing = __ballot(passes < V), weighty = __ballot(some >= 0);
+    if (passing && lane == __builtin_ctzll(passing)) atomicMin(&first_e, passes);
+    if (weighty && lane == 63 - __builtin_clzll(weighty)) atomicMax(&last_e, some);
     __syncthreads();
     if (first_e < V) break;                // (the same for all)
     run += all;
