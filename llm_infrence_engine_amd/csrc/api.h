@@ -271,13 +271,12 @@ int ms_verify_drafts(const float* p, const float* q, int n_tokens, int vocab, co
 long long ms_verify_drafts_workspace_bytes(int n_requests);      // of workspace, device memory of any contents
 void ms_verify_drafts_patience(int looks);                       // tests
 
-// pages / heads / widths / transposed: host arrays of n_tensors (at most ms_keep_tokens_max()); pages[i] [layers, num_pages,
-// heads[i], page_size, widths[i]], or [.., widths[i], page_size].  Entry first[r] + nodes[r][i] goes to first[r] + i.
+// tensors: in host memory n_tensors (at most ms_keep_tokens_max()) of {void* pages; int heads, width, transposed, 0}, pages
+// [layers, num_pages, heads, page_size, width] or [.., width, page_size].  Entry first[r] + nodes[r][i] goes to first[r] + i.
 int ms_keep_tokens_max();
-int ms_keep_tokens(void* const* pages, const int* heads, const int* widths, const int* transposed, int n_tensors, int layers,
-                   int num_pages, int page_size, const int* block_table, int table_stride, const int* table_rows,
-                   const int* first, const int* nodes, int depth, const int* counts, int n_requests, int dtype,
-                   hipStream_t stream);
+int ms_keep_tokens(const void* tensors, int n_tensors, int layers, int num_pages, int page_size, const int* block_table,
+                   int table_stride, const int* table_rows, const int* first, const int* nodes, int depth, const int* counts,
+                   int n_requests, int dtype, hipStream_t stream);
 
 // ---- mixers with a fixed-size state (csrc/sequence.hip).  A step's requests: tokens q_start[r]..q_start[r+1]-1, state
 // slot state_slots[r]; token_req [n_tokens]; n_live_tokens (may be null): tokens from there on belong to no request.

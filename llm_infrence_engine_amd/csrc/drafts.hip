@@ -375,11 +375,13 @@ verify_drafts_kernel(const float* __restrict__ p, const float* __restrict__ q, i
 // increasing, so an entry moves to an earlier place, and a place that has been written is the source of no later entry: a wave may
 // take entries in order as long as it has read a group of them before it writes that group.
 // A block works a request's moves out once (where they lie: table and pages) and its waves then walk (layer, head) pairs of one
-// tensor; with one pair a block, each of them waited for path, table and entry one after another (32 requests, 64 layers of 8 heads
-// of 128: 98 us, 1.5 TB/s).
+// tensor; where each thread did it for itself it waited for path, table and entry one after another (32 requests, 64 layers of 8
+// heads of 128 in bfloat16: 98 us).  In transposed pages an entry is one value of every row, so what has to be read and written
+// is all lines of its page's part of a head: 190 MB for those 75, 41 us as a copy takes them.  There a wave reads a row's 32 bytes
+// around the moves' places, puts the values in and writes the 32 bytes back, whole lines for memory (68 us; value by value 74).
 struct KeepTensor {
   void* pages;
-  int heads, width, transposed;
+  int heads, width, transposed, none;
 };
 struct KeepTensors { KeepTensor t[MAX_TENSORS]; };
 
@@ -399,6 +401,7 @@ keep_tokens_kernel(KeepTensors tensors, int layers, int num_pages, int page_size
   const int pairs = layers * kt.heads, width = kt.width;
   const size_t page_values = (size_t)kt.heads * page_size * width, layer_values = page_values * num_pages;
   const bool pieces = !kt.transposed && width * sizeof(T) % 16 == 0 && (uintptr_t)kt.pages % 16 == 0;
+  const bool segments = kt.transposed && page_size * sizeof(T) % 32 == 0 && (uintptr_t)kt.pages % 16 == 0;
   for (int i0 = 0; i0 < count; i0 += MS_WAVE) {
     if (wave == 0) {
       const int i = i0 + lane;
@@ -440,6 +443,37 @@ keep_tokens_kernel(KeepTensors tensors, int layers, int num_pages, int page_size
 #pragma unroll
           for (int g = 0; g < GROUP; ++g)
             if (x0 + g * MS_WAVE < total) *reinterpret_cast<uint4*>(at + to[g]) = v[g];
+        }
+      } else if (segments) {
+        constexpr int SEG = 32 / sizeof(T), GROUP = 4;      // slots of a segment, moves at a time
+        for (int m0 = 0; m0 < n;) {
+          const int page = to_page[m0], seg = to_slot[m0] / SEG;
+          int m1 = m0 + 1;
+          while (m1 < n && to_page[m1] == page && to_slot[m1] / SEG == seg) ++m1;
+          for (int e = lane; e < width; e += MS_WAVE) {
+            T* const place = at + page * page_values + (size_t)e * page_size + seg * SEG;
+            union { uint4 q[2]; T v[SEG]; } row;
+            row.q[0] = reinterpret_cast<const uint4*>(place)[0];
+            row.q[1] = reinterpret_cast<const uint4*>(place)[1];
+            for (int m = m0; m < m1; m += GROUP) {
+              T v[GROUP];
+#pragma unroll
+              for (int i = 0; i < GROUP; ++i) {
+                const int k = min(m + i, m1 - 1);
+                v[i] = at[from_page[k] * page_values + (size_t)e * page_size + from_slot[k]];
+              }
+#pragma unroll
+              for (int i = 0; i < GROUP; ++i) {
+                const int slot = __builtin_amdgcn_readfirstlane(m + i < m1 ? to_slot[m + i] % SEG : SEG);      // the same for the wave
+#pragma unroll
+                for (int k = 0; k < SEG; ++k)
+                  if (k == slot) row.v[k] = v[i];
+              }
+            }
+            reinterpret_cast<uint4*>(place)[0] = row.q[0];
+            reinterpret_cast<uint4*>(place)[1] = row.q[1];
+          }
+          m0 = m1;
         }
       } else {
         constexpr int GROUP = 8;
@@ -494,24 +528,25 @@ extern "C" int ms_verify_drafts(const float* p, const float* q, int n_tokens, in
 
 extern "C" int ms_keep_tokens_max() { return MAX_TENSORS; }
 
-extern "C" int ms_keep_tokens(void* const* pages, const int* heads, const int* widths, const int* transposed, int n_tensors,
-                              int layers, int num_pages, int page_size, const int* block_table, int table_stride,
-                              const int* table_rows, const int* first, const int* nodes, int depth, const int* counts,
-                              int n_requests, int dtype, hipStream_t stream) {
+// tensors: host memory, n_tensors of KeepTensor's 24 bytes
+extern "C" int ms_keep_tokens(const void* tensors, int n_tensors, int layers, int num_pages, int page_size, const int* block_table,
+                              int table_stride, const int* table_rows, const int* first, const int* nodes, int depth,
+                              const int* counts, int n_requests, int dtype, hipStream_t stream) {
   if (n_tensors <= 0 || n_requests <= 0 || layers <= 0) return MS_OK;
   if (n_tensors > MAX_TENSORS || num_pages <= 0 || page_size <= 0 || table_stride <= 0 || depth <= 0 || n_requests > 65535)
     return MS_BAD_ARG;
   KeepTensors ts = {};
   int most = 1;
   for (int i = 0; i < n_tensors; ++i) {
-    if (heads[i] <= 0 || widths[i] <= 0) return MS_BAD_ARG;
-    ts.t[i] = {pages[i], heads[i], widths[i], transposed[i]};
-    most = heads[i] > most ? heads[i] : most;
+    ts.t[i] = ((const KeepTensor*)tensors)[i];
+    if (ts.t[i].pages == nullptr || ts.t[i].heads <= 0 || ts.t[i].width <= 0) return MS_BAD_ARG;
+    most = std::max(most, ts.t[i].heads);
   }
   const long long pairs = (long long)layers * most;
   if (pairs > 0x3fffffffLL) return MS_UNSUPPORTED;
-  // a pair to a wave, up to sixteen waves a CU in all
-  const long long room = std::max(1LL, 16LL * ms_compute_units() / KEEP_WAVES / ((long long)n_requests * n_tensors));
+  // a pair to a wave while there are at most 128 waves a CU, four times what it holds at once: 93 us with 16, 68 with 128 (32
+  // requests, 64 layers of 8 heads of 128 in bfloat16)
+  const long long room = std::max(1LL, 128LL * ms_compute_units() / KEEP_WAVES / ((long long)n_requests * n_tensors));
   dim3 grid((unsigned)std::min((pairs + KEEP_WAVES - 1) / KEEP_WAVES, room), n_requests, n_tensors), block(KEEP_WAVES * MS_WAVE);
 #define LAUNCH(T) keep_tokens_kernel<T><<<grid, block, 0, stream>>>(ts, layers, num_pages, page_size, block_table, table_stride, table_rows, first, nodes, depth, counts)
   if (dtype == MS_F32) LAUNCH(unsigned);

@@ -131,8 +131,8 @@ _SIGNATURES = {
     "ms_verify_drafts": [_c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr,
                          _c_ptr, _c_ptr],
     "ms_keep_tokens_max": [],
-    "ms_keep_tokens": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr,
-                       _c_int, _c_ptr, _c_int, _c_int, _c_ptr],
+    "ms_keep_tokens": [_c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int,
+                       _c_ptr],
     "ms_short_conv": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_int, _c_int,
                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
     "ms_gated_delta": [_c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_int, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
@@ -1590,28 +1590,37 @@ def _tree_step(q, k_pages, v_pages, v_shape, block_table, token_req, q_start, co
     """Checks what the kernels of ``tree_attention`` have in common; the stride of q's rows and the words of a token's mask."""
     device, (P, nkv, page_size, d) = _device(), k_pages.shape
     dtype, i32 = k_pages.dtype, torch.int32
-    _code(dtype)
-    _need(k_pages, "k_pages", dtype, (P, nkv, page_size, d), device)
-    _need(v_pages, "v_pages", dtype, v_shape, device)
     stride = _rows2d(q, "q", dtype)
-    _here(q)
     N = q.shape[0]
     if q.shape[1] < num_heads * d:
         raise ValueError(f"q must be [N, >= {num_heads * d}], got {list(q.shape)}")
     if num_heads <= 0 or nkv <= 0 or num_heads % nkv:
         raise ValueError(f"{num_heads} query heads cannot share {nkv} key/value heads")
-    _need(out, "out", dtype, (N, num_heads * dv), device)
     if block_table.dim() != 2 or context_lens.dim() != 1 or tree.dim() != 2:
         raise ValueError("block_table must be [rows, pages], context_lens [requests], tree [tokens, words]")
     R, words = context_lens.shape[0], tree.shape[1]
-    _need(block_table, "block_table", i32, tuple(block_table.shape), device)
-    _need(context_lens, "context_lens", i32, (R,), device)
-    _need(q_start, "q_start", i32, (R + 1,), device)
-    _need(token_req, "token_req", i32, (N,), device)
-    _need(tree, "tree", i32, (N, words), device)
-    if table_rows is not None:
-        _need(table_rows, "table_rows", i32, (R,), device)
-    elif block_table.shape[0] < R:
+    # everything at once (2 us); one by one, for the message, only where something does not fit
+    tables = (block_table, context_lens, q_start, token_req, tree) if table_rows is None else (block_table, context_lens, q_start, token_req, tree, table_rows)
+    fits = q.get_device() == device and q_start.shape == (R + 1,) and token_req.shape == (N,) and tree.shape == (N, words) and \
+        v_pages.shape == v_shape and out.shape == (N, num_heads * dv) and (table_rows is None or table_rows.shape == (R,))
+    for t in tables:
+        fits = fits and t.dtype is i32 and t.get_device() == device and t.is_contiguous()
+    for t in (k_pages, v_pages, out):
+        fits = fits and t.dtype is dtype and t.get_device() == device and t.is_contiguous()
+    if not fits:
+        _code(dtype)
+        _here(q)
+        _need(k_pages, "k_pages", dtype, (P, nkv, page_size, d), device)
+        _need(v_pages, "v_pages", dtype, v_shape, device)
+        _need(out, "out", dtype, (N, num_heads * dv), device)
+        _need(block_table, "block_table", i32, tuple(block_table.shape), device)
+        _need(context_lens, "context_lens", i32, (R,), device)
+        _need(q_start, "q_start", i32, (R + 1,), device)
+        _need(token_req, "token_req", i32, (N,), device)
+        _need(tree, "tree", i32, (N, words), device)
+        if table_rows is not None:
+            _need(table_rows, "table_rows", i32, (R,), device)
+    if table_rows is None and block_table.shape[0] < R:
         raise ValueError(f"the block table has {block_table.shape[0]} rows for {R} requests")
     if max_q_len < 1:
         raise ValueError(f"max_q_len {max_q_len}: a tree has at least one token")
@@ -1677,6 +1686,10 @@ def verify_drafts(p: torch.Tensor, q: Optional[torch.Tensor], token_ids: torch.T
     return out
 
 
+MAX_KEPT_TENSORS = 16      # page tensors one call of ``keep_tokens`` takes (the library's ms_keep_tokens_max)
+_KEPT_TENSOR = struct.Struct("Qiiii")
+
+
 def keep_tokens(pages, transposed, block_table: torch.Tensor, first: torch.Tensor, nodes: torch.Tensor, counts: torch.Tensor,
                 table_rows: Optional[torch.Tensor] = None) -> None:
     """Moves what an accepted path stored together: entry first[r] + nodes[r, i] of request r becomes entry first[r] + i, for
@@ -1684,12 +1697,11 @@ def keep_tokens(pages, transposed, block_table: torch.Tensor, first: torch.Tenso
     [layers, pages, heads, width, page_size] where ``transposed`` says so (or without the layers).  ``first`` int32 [R]: the
     entry of the step's first token (context length less tokens); ``nodes`` int32 [R, depth] and ``counts`` int32 [R] as
     ``verify_drafts`` leaves them: increasing, 0 first.  Entries whose page is the null page or outside the pool stay."""
-    pages, transposed = list(pages), list(transposed)
-    if not pages or len(pages) != len(transposed):
+    n = len(pages)
+    if n == 0 or n != len(transposed):
         raise ValueError("one or more page tensors, and for each whether it is transposed")
-    most = _get("ms_keep_tokens_max")()
-    if len(pages) > most:
-        raise ValueError(f"at most {most} page tensors to a call")
+    if n > MAX_KEPT_TENSORS:
+        raise ValueError(f"at most {MAX_KEPT_TENSORS} page tensors to a call")
     device, i32 = _device(), torch.int32
     if nodes.dim() != 2 or block_table.dim() != 2:
         raise ValueError("nodes must be [requests, depth], block_table [rows, pages]")
@@ -1702,26 +1714,28 @@ def keep_tokens(pages, transposed, block_table: torch.Tensor, first: torch.Tenso
         _need(table_rows, "table_rows", i32, (R,), device)
     elif block_table.shape[0] < R:
         raise ValueError(f"the block table has {block_table.shape[0]} rows for {R} requests")
-    sizes = []
+    dtype = pages[0].dtype
+    code = _code(dtype)
+    sizes, record = None, b""
     for t, flip in zip(pages, transposed):
-        _need(t, "pages", pages[0].dtype, tuple(t.shape), device)
-        if t.dim() not in (4, 5):
-            raise ValueError(f"pages must be [layers, pages, heads, page size, width] or without the layers, got {list(t.shape)}")
-        L, P, heads, a, b = t.shape if t.dim() == 5 else (1, *t.shape)
-        sizes.append((L, P, b if flip else a, heads, a if flip else b))
-    if any(s[:3] != sizes[0][:3] for s in sizes):
-        raise ValueError("the page tensors of a call have the same layers, pages and page size")
-    L, P, page_size = sizes[0][:3]
-    code = _code(pages[0].dtype)
-    if R == 0 or depth == 0 or L == 0 or P == 0:
+        shape = tuple(t.shape)
+        _need(t, "pages", dtype, shape, device)
+        if len(shape) not in (4, 5):
+            raise ValueError(f"pages must be [layers, pages, heads, page size, width] or without the layers, got {list(shape)}")
+        L, P, heads, a, b = shape if len(shape) == 5 else (1, *shape)
+        page_size, width = (b, a) if flip else (a, b)
+        if sizes is None:
+            sizes = (L, P, page_size)
+        elif sizes != (L, P, page_size):
+            raise ValueError("the page tensors of a call have the same layers, pages and page size")
+        record += _KEPT_TENSOR.pack(t.data_ptr(), heads, width, bool(flip), 0)
+    if R == 0 or depth == 0 or 0 in pages[0].shape:
         return
     if R > 65535:
         raise ValueError("at most 65,535 requests to a call")
-    keep, ptrs = _pointer_array(pages)
-    n = len(pages)
-    ints = [(_c_int * n)(*v) for v in ([s[3] for s in sizes], [s[4] for s in sizes], [int(bool(f)) for f in transposed])]
-    _call("ms_keep_tokens", ptrs, *(ctypes.cast(a, ctypes.c_void_p) for a in ints), n, L, P, page_size, block_table.data_ptr(),
-          block_table.shape[1], _ptr(table_rows), first.data_ptr(), nodes.data_ptr(), depth, counts.data_ptr(), R, code, _stream())
+    L, P, page_size = sizes
+    _call("ms_keep_tokens", record, n, L, P, page_size, block_table.data_ptr(), block_table.shape[1], _ptr(table_rows), first.data_ptr(),
+          nodes.data_ptr(), depth, counts.data_ptr(), R, code, _stream())
 
 
 # ------------------------------------------------------------------------------------------------ state-carrying mixers

@@ -770,7 +770,7 @@ def host(monkeypatch):
     monkeypatch.setattr(ops, "_device", lambda: -1)
     monkeypatch.setattr(ops, "_call", lambda name, *a: launched.append(name))
     monkeypatch.setattr(ops, "_stream", lambda: 0)
-    monkeypatch.setattr(ops, "_get", lambda name: (lambda *a: {"ms_keep_tokens_max": 16}.get(name, 64)))      # (sizes of workspaces)
+    monkeypatch.setattr(ops, "_get", lambda name: (lambda *a: 64))      # (sizes of workspaces)
     return launched
 
 
@@ -789,6 +789,11 @@ def test_ops_of_trees_run_on_the_gpu_only():
         ops.verify_drafts(z, None, i, i, i, z[:, 0], i.view(1, 2), i[:1], i[:1])
     with pytest.raises(RuntimeError):
         ops.keep_tokens([torch.zeros(2, 2, 2, 2)], [False], i.view(1, 2), i[:1], i.view(1, 2), i[:1])
+
+
+@gpu
+def test_the_library_takes_as_many_tensors_as_the_module_says():
+    assert ops._get("ms_keep_tokens_max")() == ops.MAX_KEPT_TENSORS
 
 
 def test_probabilities_refuse(host):
