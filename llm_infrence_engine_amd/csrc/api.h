@@ -263,6 +263,16 @@ int ms_tree_attention_mfma(const void* q, long long q_stride, const void* k_page
                            void* part_ml, int n_requests, int n_tokens, int max_q_len, int num_heads, int num_kv_heads,
                            int head_dim, int page_size, float scale, int kind, int share, int n_splits, hipStream_t stream);
 
+// And for float: values as keys, pages of any size.  ms_tree_attention_f32_share: the keys a block takes (0: not its sizes); n_splits:
+// how many blocks the longest context then has.
+int ms_tree_attention_f32_share(int n_requests, int n_tokens, int max_q_len, int max_context_len, int num_heads, int num_kv_heads,
+                                int head_dim);
+int ms_tree_attention_f32(const float* q, long long q_stride, const float* k_pages, const float* v_pages, const int* block_table,
+                          int table_stride, const int* table_rows, const int* token_req, const int* q_start, const int* context_lens,
+                          const int* tree, int words, float* out, long long out_stride, float* part_o, float* part_ml, int n_requests,
+                          int n_tokens, int max_q_len, int num_heads, int num_kv_heads, int head_dim, int page_size, long long num_pages,
+                          float scale, int share, int n_splits, hipStream_t stream);
+
 // p, q [n_tokens, vocab] (q may be null), tokens / parents / uniforms [n_tokens], q_start [n_requests + 1] -> nodes
 // [n_requests, depth] (the accepted path, -1 behind it), counts [n_requests], out [n_requests] (the token drawn behind it).
 int ms_verify_drafts(const float* p, const float* q, int n_tokens, int vocab, const int* tokens, const int* parents,

@@ -16,6 +16,7 @@
 #include "attention_tiles.h"
 #include "api.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -416,10 +417,10 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
 // head): a split's reference and sum to a lane, then every lane its dims of one split after another.
 constexpr int COMBINE_WAVES = 4, AT_ONCE = 8;      // (parts a lane asks for at a time)
 
-template <int D>
+template <typename T, int D>
 __global__ void __launch_bounds__(COMBINE_WAVES * MS_WAVE)
 tree_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ token_req,
-                    const int* __restrict__ q_start, const int* __restrict__ context_lens, int n_requests, bf16* __restrict__ out,
+                    const int* __restrict__ q_start, const int* __restrict__ context_lens, int n_requests, T* __restrict__ out,
                     size_t out_stride, int n_tokens, int nh, int share, int n_splits) {
   constexpr int DL = (D + MS_WAVE - 1) / MS_WAVE;
   const int lane = threadIdx.x & (MS_WAVE - 1);
@@ -463,7 +464,231 @@ tree_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ 
   const float inv = den != 0.f ? 1.0f / den : 0.f;
 #pragma unroll
   for (int e = 0; e < DL; ++e)
-    if (lane + e * MS_WAVE < D) out[(size_t)n * out_stride + (size_t)h * D + lane + e * MS_WAVE] = __float2bfloat16(acc[e] * inv);
+    if (lane + e * MS_WAVE < D) out[(size_t)n * out_stride + (size_t)h * D + lane + e * MS_WAVE] = from_float<T>(acc[e] * inv);
+}
+
+// ---- the 32-bit path (v_mfma_f32_16x16x4_f32): scores, exponentials, weights and values are floats.  A wave owns NT tiles of 16
+// columns and takes every F32_WAVES-th tile of 16 keys of the block's share, with the next one's keys and values on their way in
+// registers; the waves merge through LDS, each its part of the dims.  A step of the score product takes one entry of each of four
+// quarters of 16 dims, and one of the value product one key of each of four quarters of 16, so that a lane reads 16 bytes of its
+// key's row and has its own keys' weights where they are: O^T[dim, col] += V^T[dim, key] . P^T[key, col].  Pages may have any size.
+// 157 TFLOP/s are more than it can be fed: it waits for its loads (6 trees of up to 13 tokens behind 700 keys, 14 heads of 64 on 2:
+// 60 us on the vector ALUs, which read every key for every column).
+constexpr int F32_WAVES = 8;
+
+template <int D, int NT>
+__global__ void __launch_bounds__(F32_WAVES * MS_WAVE, 2)
+tree_attention_f32_kernel(const float* __restrict__ q, size_t q_stride, const float* __restrict__ k_pages,
+                          const float* __restrict__ v_pages, const int* __restrict__ block_table, int table_stride,
+                          const int* __restrict__ table_rows, const int* __restrict__ q_start, const int* __restrict__ context_lens,
+                          const unsigned* __restrict__ tree, int words, float* __restrict__ out, size_t out_stride,
+                          float* __restrict__ part_o, float* __restrict__ part_ml, int nh, int nkv, int page_size, int page_shift,
+                          float scale_log2e, int n_requests, int n_splits, int share) {
+  constexpr int CT = D / 16, COLS = NT * 16;
+  extern __shared__ __align__(16) unsigned char lds_raw[];
+  f32x4* sm_o = reinterpret_cast<f32x4*>(lds_raw);       // [wave][tile of dims][NT][64]
+  __shared__ float sm_m[F32_WAVES][COLS], sm_l[F32_WAVES][COLS];
+  const int lane = threadIdx.x & (MS_WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / MS_WAVE);
+  const int col16 = lane & 15, kq = lane >> 4;
+  const int g = blockIdx.x, rep = nh / nkv, split = blockIdx.z;
+  int r, tile, n_tiles;
+  if (n_requests == 0) {
+    r = blockIdx.y; tile = 0;
+  } else {
+    find_tile(q_start, n_requests, rep, COLS, blockIdx.y, lane, r, tile, n_tiles);
+    if (r < 0) return;
+  }
+  const int* table = block_table + (size_t)(table_rows ? table_rows[r] : r) * table_stride;
+  const int q0 = q_start[r], qlen = q_start[r + 1] - q0, context = context_lens[r], before = context - qlen, ncols = qlen * rep;
+  const int t_begin = split * (share / 16), t_end = min((context + 15) / 16, t_begin + share / 16);
+  if (t_begin >= t_end || qlen <= 0) return;
+
+  // the row of the lane's key of a tile among all rows of keys (of values the same); past the context: the last one's
+  auto row_of = [&](int t) {
+    const int key = min(t * 16 + col16, context - 1), page = page_shift >= 0 ? key >> page_shift : key / page_size;
+    return (table[page] * nkv + g) * page_size + (key - page * page_size);
+  };
+  // at 128 dims there are no registers for the next tile's values beside its keys: they are asked for where a tile's turn begins
+  constexpr bool VALUES_EARLY = D < 128;
+  float4 k[2][CT];
+  float v[VALUES_EARLY ? 2 : 1][CT][4];
+  auto load_keys = [&](int row, float4 (&kf)[CT]) __attribute__((always_inline)) {
+    const float* kp = k_pages + (size_t)row * D + kq * 4;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) kf[c] = *reinterpret_cast<const float4*>(kp + c * 16);
+  };
+  auto load_values = [&](int row, float (&vf)[CT][4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* vp = v_pages + (size_t)__shfl(row, kq * 4 + i, MS_WAVE) * D + col16;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) vf[c][i] = vp[c * 16];
+    }
+  };
+  int row_now = 0, row_next = 0;
+  if (t_begin + wave < t_end) {
+    row_now = row_of(t_begin + wave);
+    load_keys(row_now, k[0]);
+    if (VALUES_EARLY) load_values(row_now, v[0]);
+  }
+  if (t_begin + wave + F32_WAVES < t_end) row_next = row_of(t_begin + wave + F32_WAVES);
+
+  bool idle[NT];
+  float4 qv[NT][CT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int c = tile * COLS + t * 16 + col16, cc = min(c, ncols - 1);
+    idle[t] = c >= ncols;
+    const float* qp = q + (size_t)(q0 + cc / rep) * q_stride + (size_t)(g * rep + cc % rep) * D + kq * 4;
+#pragma unroll
+    for (int j = 0; j < CT; ++j) qv[t][j] = *reinterpret_cast<const float4*>(qp + j * 16);
+  }
+  // which of the keys base + kq * 4 + (0..3) column tile t sees
+  auto visible = [&](int t, int base) -> unsigned {
+    const int rel = base + kq * 4 - before;
+    if (idle[t]) return 0u;
+    if (rel <= -4) return 0xfu;
+    const unsigned* mask = tree + (size_t)(q0 + min(tile * COLS + t * 16 + col16, ncols - 1) / rep) * words;
+    const int at = max(rel, 0), w = at >> 5;
+    const unsigned lo = w < words ? mask[w] : 0u, hi = w + 1 < words ? mask[w + 1] : 0u;
+    unsigned bits = (unsigned)((((unsigned long long)hi << 32) | lo) >> (at & 31)) & 0xfu;
+    if (rel < 0) bits = ((bits << -rel) | ((1u << -rel) - 1u)) & 0xfu;
+    const int left = qlen - rel;
+    return left >= 4 ? bits : left <= 0 ? 0u : bits & ((1u << left) - 1u);
+  };
+  float m[NT], l[NT];
+  f32x4 o[CT][NT] = {};
+#pragma unroll
+  for (int t = 0; t < NT; ++t) { m[t] = -INFINITY; l[t] = 0.f; }
+
+  auto step = [&](int t, float4 (&kf)[CT], float (&vf)[CT][4], float4 (&kn)[CT], float (&vn)[CT][4]) __attribute__((always_inline)) {
+    if (!VALUES_EARLY) load_values(row_now, vf);
+    if (t + F32_WAVES < t_end) {
+      load_keys(row_next, kn);
+      if (VALUES_EARLY) load_values(row_next, vn);
+      row_now = row_next;
+      if (t + 2 * F32_WAVES < t_end) row_next = row_of(t + 2 * F32_WAVES);
+    }
+    const int base = t * 16;
+    f32x4 s[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < CT; ++j)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].x, qv[n][j].x, s[n], 0, 0, 0);
+        s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].y, qv[n][j].y, s[n], 0, 0, 0);
+        s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].z, qv[n][j].z, s[n], 0, 0, 0);
+        s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].w, qv[n][j].w, s[n], 0, 0, 0);
+      }
+    const bool masked = base + 16 > before;
+    unsigned sees[NT];
+    bool spoiled = false;
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        sees[n] = visible(n, base);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = (sees[n] >> i) & 1u ? s[n][i] : -INFINITY;
+      }
+      // (as in the kernel above: what no column may meet, and what not every column may)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = base + kq * 4 + i;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          const bool gone = key >= context, wild = (key >= before) & !(fabsf(vf[c][i]) < INFINITY) & !gone;
+          spoiled |= wild;
+          vf[c][i] = gone | wild ? 0.f : vf[c][i];
+        }
+      }
+    }
+    f32x4 p[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float top = fmaxf(m[n], column_max(fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3]))) * scale_log2e);
+      const float ref = top == -INFINITY ? 0.f : top, corr = fast_exp2(m[n] - ref);      // 0 while nothing has been seen
+      m[n] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[n][i] = fast_exp2(fmaf(s[n][i], scale_log2e, -ref));
+        sum += p[n][i];
+      }
+      l[n] = fmaf(l[n], corr, sum);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) o[c][n] *= corr;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[c][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[c][i], p[n][i], o[c][n], 0, 0, 0);
+    if (masked && __builtin_amdgcn_ballot_w64(spoiled) != 0) {
+      int dims = D;
+      for (int x = 0; x < 16; ++x) {
+        const int key = base + x;
+        if (key < before || key >= context) continue;
+        const int page = key / page_size, owner = (x >> 2) * 16 + col16;
+        const float* from = v_pages + ((size_t)table[page] * nkv + g) * page_size * D + (size_t)(key - page * page_size) * D;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float w = __shfl((x & 3) == 0 ? p[n][0] : (x & 3) == 1 ? p[n][1] : (x & 3) == 2 ? p[n][2] : p[n][3], owner, MS_WAVE);
+          const bool see = (__shfl(sees[n], owner, MS_WAVE) >> (x & 3)) & 1u;
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            asm volatile("" : "+s"(dims) : : "memory");
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float value = from[min(c * 16 + kq * 4 + i, dims - 1)];
+              if (see && !(fabsf(value) < INFINITY)) o[c][n][i] += w * value;
+            }
+          }
+        }
+      }
+    }
+  };
+  for (int t = t_begin + wave; t < t_end; t += 2 * F32_WAVES) {
+    step(t, k[0], v[0], k[1], v[VALUES_EARLY]);
+    if (t + F32_WAVES < t_end) step(t + F32_WAVES, k[1], v[VALUES_EARLY], k[0], v[0]);
+  }
+
+  // every wave merges every F32_WAVES-th (tile of dims, tile of columns)
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    l[t] += __shfl_xor(l[t], 16, MS_WAVE);
+    l[t] += __shfl_xor(l[t], 32, MS_WAVE);
+    if (kq == 0) { sm_m[wave][t * 16 + col16] = m[t]; sm_l[wave][t * 16 + col16] = l[t]; }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) sm_o[((wave * CT + c) * NT + t) * MS_WAVE + lane] = o[c][t];
+  }
+  __syncthreads();
+  for (int part = wave; part < CT * NT; part += F32_WAVES) {
+    const int c = part / NT, t = part - c * NT;
+    float big = -INFINITY, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < F32_WAVES; ++w) big = fmaxf(big, sm_m[w][t * 16 + col16]);
+    const float safe = big == -INFINITY ? 0.f : big;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < F32_WAVES; ++w) {
+      const float f = fast_exp2(sm_m[w][t * 16 + col16] - safe);
+      den = fmaf(sm_l[w][t * 16 + col16], f, den);
+      sum += sm_o[((w * CT + c) * NT + t) * MS_WAVE + lane] * f;
+    }
+    const int col = tile * COLS + t * 16 + col16;
+    if (col >= ncols) continue;
+    const int tok = q0 + col / rep, head = g * rep + col % rep;
+    if (n_splits > 1) {
+      const size_t slot = ((size_t)tok * nh + head) * n_splits + split;
+      *reinterpret_cast<f32x4*>(part_o + slot * D + c * 16 + kq * 4) = sum;
+      if (c == 0 && kq == 0) { part_ml[slot * 2] = big; part_ml[slot * 2 + 1] = den; }
+    } else {
+      *reinterpret_cast<f32x4*>(out + (size_t)tok * out_stride + (size_t)head * D + c * 16 + kq * 4) = sum * (den != 0.f ? 1.0f / den : 0.f);
+    }
+  }
 }
 
 struct Call {
@@ -505,7 +730,7 @@ int launch(const Call& a) {
       a.part_ml, a.nh, a.nkv, a.page_size, page_shift_of(a.page_size), a.scale_log2e, one ? 0 : a.n_requests, a.n_splits, a.share / S::KEYS);
   if (a.n_splits > 1) {
     const long long items = (long long)a.n_tokens * a.nh;
-    tree_combine_kernel<D><<<dim3((unsigned)((items + COMBINE_WAVES - 1) / COMBINE_WAVES)), dim3(COMBINE_WAVES * MS_WAVE), 0, a.stream>>>(
+    tree_combine_kernel<bf16, D><<<dim3((unsigned)((items + COMBINE_WAVES - 1) / COMBINE_WAVES)), dim3(COMBINE_WAVES * MS_WAVE), 0, a.stream>>>(
         a.part_o, a.part_ml, a.token_req, a.q_start, a.ctx, a.n_requests, a.out, a.out_stride, a.n_tokens, a.nh, a.share, a.n_splits);
   }
   return ms_launch_status();
@@ -586,5 +811,64 @@ extern "C" int ms_tree_attention_mfma(const void* q, long long q_stride, const v
   if (head_dim == 64) GO(64, 2);
   if (head_dim == 128) GO(128, 1);
 #undef GO
+  return MS_UNSUPPORTED;
+}
+
+// Keys that a block of the 32-bit kernel takes, for a step of these sizes (all bounds); 0: sizes it does not take.  About a block a
+// CU, but never less than a tile for every wave: a block's turns of F32_WAVES tiles come one after another, 1 us each.
+extern "C" int ms_tree_attention_f32_share(int n_requests, int n_tokens, int max_q_len, int max_context_len, int num_heads,
+                                           int num_kv_heads, int head_dim) {
+  if ((head_dim != 32 && head_dim != 64 && head_dim != 128) || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads) return 0;
+  if (n_requests <= 0 || n_tokens <= 0 || max_q_len <= 0) return 0;
+  const int rep = num_heads / num_kv_heads, turn = 16 * F32_WAVES;
+  if ((long long)max_q_len * rep > 0x3fffffffLL) return 0;
+  const long long blocks = column_tiles(n_requests, n_tokens, max_q_len, rep, head_dim == 128 ? 16 : 32) * num_kv_heads;
+  const long long context = std::max(1, max_context_len), turns = (context + turn - 1) / turn;
+  const long long splits = std::max(1LL, std::min({turns, (long long)MAX_SPLITS, ms_compute_units() / blocks}));
+  return (int)((turns + splits - 1) / splits * turn);
+}
+
+// As ms_tree_attention_mfma, for float: values [P, nkv, page_size, head_dim], pages of any size; num_pages: rows are counted in an int.
+extern "C" int ms_tree_attention_f32(const float* q, long long q_stride, const float* k_pages, const float* v_pages,
+                                     const int* block_table, int table_stride, const int* table_rows, const int* token_req,
+                                     const int* q_start, const int* context_lens, const int* tree, int words, float* out,
+                                     long long out_stride, float* part_o, float* part_ml, int n_requests, int n_tokens, int max_q_len,
+                                     int num_heads, int num_kv_heads, int head_dim, int page_size, long long num_pages, float scale,
+                                     int share, int n_splits, hipStream_t stream) {
+  if (n_requests <= 0 || n_tokens <= 0 || max_q_len <= 0) return MS_OK;
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || table_stride <= 0 || words <= 0 || page_size <= 0) return MS_BAD_ARG;
+  if (!(scale > 0.f)) return MS_UNSUPPORTED;   // maxima are taken of the raw scores
+  if (share <= 0 || share % 16 || n_splits < 1 || n_splits > MAX_SPLITS || (n_splits > 1 && (part_o == nullptr || part_ml == nullptr))) return MS_BAD_ARG;
+  if (num_kv_heads > 65535 || num_pages * num_kv_heads * page_size >= (1ll << 31)) return MS_UNSUPPORTED;
+  if (q_stride % 4 || out_stride % 4 || ((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pages | (uintptr_t)part_o) % 16) return MS_UNSUPPORTED;
+  const int rep = num_heads / num_kv_heads;
+  if ((long long)max_q_len * rep > 0x3fffffffLL || (long long)n_tokens * num_heads > 0x3fffffffLL) return MS_UNSUPPORTED;
+  auto go = [&](auto dims, auto nt) {
+    constexpr int D = decltype(dims)::value, NT = decltype(nt)::value;
+    constexpr int lds = F32_WAVES * (D / 16) * NT * MS_WAVE * (int)sizeof(f32x4);
+    static bool raised = false;   // once per instantiation: allow more LDS than the default 64 KB
+    if (!raised) {
+      if (hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_attention_f32_kernel<D, NT>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+        return (int)MS_LAUNCH_FAILED;
+      raised = true;
+    }
+    const bool one = (long long)max_q_len * rep <= NT * 16;
+    const long long tiles = one ? n_requests : column_tiles(n_requests, n_tokens, max_q_len, rep, NT * 16);
+    if (tiles > 65535) return (int)MS_UNSUPPORTED;
+    tree_attention_f32_kernel<D, NT><<<dim3(num_kv_heads, (unsigned)tiles, n_splits), dim3(F32_WAVES * MS_WAVE), lds, stream>>>(
+        q, (size_t)q_stride, k_pages, v_pages, block_table, table_stride, table_rows, q_start, context_lens, (const unsigned*)tree, words, out,
+        (size_t)out_stride, part_o, part_ml, num_heads, num_kv_heads, page_size, page_shift_of(page_size), scale * 1.4426950408889634f,
+        one ? 0 : n_requests, n_splits, share);
+    if (n_splits > 1) {
+      const long long items = (long long)n_tokens * num_heads;
+      tree_combine_kernel<float, D><<<dim3((unsigned)((items + COMBINE_WAVES - 1) / COMBINE_WAVES)), dim3(COMBINE_WAVES * MS_WAVE), 0, stream>>>(
+          part_o, part_ml, token_req, q_start, context_lens, n_requests, out, (size_t)out_stride, n_tokens, num_heads, share, n_splits);
+    }
+    return ms_launch_status();
+  };
+  if (head_dim == 32) return go(std::integral_constant<int, 32>{}, std::integral_constant<int, 2>{});
+  if (head_dim == 64) return go(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+  if (head_dim == 128) return go(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{});
   return MS_UNSUPPORTED;
 }

@@ -126,6 +126,10 @@ _SIGNATURES = {
     "ms_tree_attention_mfma_plan": [_c_int] * 8,
     "ms_tree_attention_mfma": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr,
                                _c_ll, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int, _c_ptr],
+    "ms_tree_attention_f32_share": [_c_int] * 7,
+    "ms_tree_attention_f32": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr,
+                              _c_ll, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ll, _c_float, _c_int,
+                              _c_int, _c_ptr],
     "ms_verify_drafts_workspace_bytes": [_c_int],
     "ms_verify_drafts_patience": [_c_int],
     "ms_verify_drafts": [_c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr,
@@ -1557,32 +1561,42 @@ def tree_attention_generic(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     return out
 
 
-def tree_attention_mfma(q: torch.Tensor, k_pages: torch.Tensor, vt_pages: torch.Tensor, block_table: torch.Tensor,
+def tree_attention_mfma(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                         token_req: torch.Tensor, q_start: torch.Tensor, context_lens: torch.Tensor, tree: torch.Tensor,
                         out: torch.Tensor, num_heads: int, scale: float, max_q_len: int, max_context_len: int,
                         table_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``tree_attention`` on the matrix cores: bfloat16, heads of 32, 64 or 128 entries, value pages of that size transposed,
-    pages of a multiple of 16 tokens, a positive scale.  ``max_q_len`` and ``max_context_len`` are upper bounds; tokens from
-    q_start[R] on belong to no request, a request may have no token."""
-    if k_pages.dtype != torch.bfloat16 or k_pages.dim() != 4:
-        raise TypeError("pages must be bfloat16, [pages, heads, page size, width]")
+    """``tree_attention`` on the matrix cores: heads of 32, 64 or 128 entries, keys and values of one size, a positive scale;
+    bfloat16 with value pages transposed and pages of a multiple of 16 tokens, or float32 with value pages as the keys', of
+    any size.  ``max_q_len`` and ``max_context_len`` are upper bounds; tokens from q_start[R] on belong to no request, a
+    request may have no token."""
+    if k_pages.dim() != 4:
+        raise ValueError("pages must be [pages, heads, page size, width]")
     P, nkv, page_size, d = k_pages.shape
-    q_stride, words = _tree_step(q, k_pages, vt_pages, (P, nkv, d, page_size), block_table, token_req, q_start, context_lens, tree, table_rows, out,
-                                 num_heads, d, max_q_len)
+    small = k_pages.dtype == torch.bfloat16
+    q_stride, words = _tree_step(q, k_pages, v_pages, (P, nkv, d, page_size) if small else (P, nkv, page_size, d), block_table, token_req,
+                                 q_start, context_lens, tree, table_rows, out, num_heads, d, max_q_len)
     N, R = q.shape[0], context_lens.shape[0]
     if N == 0 or R == 0:
         return out
-    plan = _get("ms_tree_attention_mfma_plan")(R, N, max_q_len, max_context_len, num_heads, nkv, d, page_size)
-    kind, share = (plan >> 16, (plan & 0xFFFF) * 64) if plan >= 0 else (0, 64)
+    if small:
+        plan = _get("ms_tree_attention_mfma_plan")(R, N, max_q_len, max_context_len, num_heads, nkv, d, page_size)
+        kind, share = plan >> 16, (plan & 0xFFFF) * 64
+    else:
+        kind, share = 0, _get("ms_tree_attention_f32_share")(R, N, max_q_len, max_context_len, num_heads, nkv, d)
+    if kind < 0 or share <= 0:
+        raise UnsupportedShape(f"the matrix-core attention over trees takes heads of 32, 64 and 128, not {d} (pages of {page_size})")
     n_splits = -(-max_context_len // share)
     part_o = part_ml = None
     if n_splits > 1:
         parts = torch.empty(N * num_heads * n_splits * (d + 2), dtype=torch.float32, device=q.device)
         part_o, part_ml = parts.data_ptr(), parts.data_ptr() + 4 * N * num_heads * n_splits * d
-    _call("ms_tree_attention_mfma", q.data_ptr(), q_stride, k_pages.data_ptr(), vt_pages.data_ptr(), block_table.data_ptr(),
-          block_table.shape[1], _ptr(table_rows), token_req.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(), tree.data_ptr(),
-          words, out.data_ptr(), num_heads * d, part_o, part_ml, R, N, max_q_len, num_heads, nkv, d, page_size, float(scale),
-          kind, share, n_splits, _stream())
+    args = (q.data_ptr(), q_stride, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), block_table.shape[1], _ptr(table_rows),
+            token_req.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(), tree.data_ptr(), words, out.data_ptr(), num_heads * d,
+            part_o, part_ml, R, N, max_q_len, num_heads, nkv, d, page_size)
+    if small:
+        _call("ms_tree_attention_mfma", *args, float(scale), kind, share, n_splits, _stream())
+    else:
+        _call("ms_tree_attention_f32", *args, P, float(scale), share, n_splits, _stream())
     return out
 
 
@@ -1637,9 +1651,13 @@ def tree_attention(q: torch.Tensor, kv, ctx, tree: torch.Tensor, out: torch.Tens
     The step's keys and values lie in the cache in the order of the tokens (``slot_mapping``), encoded with whatever
     positions the tree gives them; ``keep_tokens`` moves together what is accepted."""
     d, page_size = kv.k_pages.shape[3], kv.k_pages.shape[2]
-    if (q.dtype == torch.bfloat16 and kv.v_transposed and kv.v_pages.shape[2] == d and attention_mfma_supported(d, page_size) and scale > 0
-            and kv.k_pages.data_ptr() % 16 == 0 and kv.v_pages.data_ptr() % 16 == 0 and q.data_ptr() % 16 == 0
-            and out.data_ptr() % 8 == 0 and (q.shape[0] == 1 or q.stride(0) % 8 == 0)):
+    dv = kv.v_pages.shape[2] if kv.v_transposed else kv.v_pages.shape[3]
+    if q.dtype == torch.bfloat16:
+        takes, per = kv.v_transposed and page_size % 16 == 0, 8
+    else:
+        takes, per = not kv.v_transposed and kv.k_pages.shape[0] * kv.k_pages.shape[1] * page_size < 1 << 31, 4
+    if takes and d == dv and d in (32, 64, 128) and scale > 0 and (q.shape[0] == 1 or q.stride(0) % per == 0) and \
+            (kv.k_pages.data_ptr() | kv.v_pages.data_ptr() | q.data_ptr() | out.data_ptr()) % 16 == 0:
         return tree_attention_mfma(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.q_start, ctx.context_lens, tree, out,
                                    num_heads, scale, max(1, ctx.max_q_len), max(1, ctx.max_context_len), kv.table_rows)
     return tree_attention_generic(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.q_start, ctx.context_lens, tree,
