@@ -80,6 +80,20 @@ class CachePools:
         """Table entries that changed, as the cache manager's ``take_updates`` lists them (device tensors)."""
         ops.table_update(self.tables, list(index), list(value), counts, max_updates)
 
+    def keep_tokens(self, first: torch.Tensor, nodes: torch.Tensor, counts: torch.Tensor, table_rows: torch.Tensor) -> None:
+        """Moves what an accepted path of drafted tokens stored together, in every group's pages (``ops.keep_tokens``): entry
+        first[r] + nodes[r, i] of the step's request r, whose row is ``table_rows[r]``, to first[r] + i for i < counts[r].  A
+        state that has seen a token, or an entry that stands for several, cannot lose it again: such caches are refused."""
+        if self.state:
+            raise ValueError("a cache with per-request state cannot drop tokens that its state has seen")
+        if any(key.stride != 1 for key in self.layout.group_keys):
+            raise ValueError("a cache with entries for whole blocks of tokens cannot drop tokens of a block")
+        for pages, flipped, table in zip(self.pages, self.transposed, self.tables):
+            names = list(pages)
+            for i in range(0, len(names), ops.MAX_KEPT_TENSORS):
+                some = names[i:i + ops.MAX_KEPT_TENSORS]
+                ops.keep_tokens([pages[n] for n in some], [flipped[n] for n in some], table, first, nodes, counts, table_rows)
+
     def state_view(self, run: int) -> StateView:
         need = self.layout.state_needs[run]
         return StateView(self.state[run] if isinstance(need, tuple) else self.state[run][0])

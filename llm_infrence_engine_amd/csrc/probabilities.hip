@@ -37,8 +37,9 @@ struct RowWork {                       // one per row, in the workspace the call
   unsigned n_candidates, n_ties;       // ties: values equal to the bound
   unsigned bound;                      // top-k: every value above it is a candidate
   int bin;                             // top-p alone: the middle bin of the candidates, < 0: none
-  unsigned long long chunk_mass[MAX_CHUNKS];    // (no temperature: where the largest stands)
-  unsigned long long chunk_above[MAX_CHUNKS];   // mass of the values above the candidates'
+  double chunk_mass[MAX_CHUNKS];
+  double chunk_above[MAX_CHUNKS];      // mass of the values above the candidates'
+  int chunk_first[MAX_CHUNKS];         // no temperature: where the largest stands
   unsigned candidates[MAX_CANDIDATES];          // keys
   float hist[BINS];
   unsigned groups[MAX_CHUNKS * WAVES * 4];
@@ -120,22 +121,22 @@ __device__ __forceinline__ float exp_of(float x) {
   return fmaf(e * 0.693147181f, r, e);
 }
 
-// e^(s - zmax) cut to 44 binary places, in two words of 20 and 24 (a conversion to 64 bits at once is three times as long).
-struct Mass {
-  unsigned hi, lo;
-  __device__ __forceinline__ explicit Mass(float e) {
-    const float scaled = e * (float)(1u << (FIX_PLACES - 24));
-    hi = (unsigned)scaled;
-    lo = (unsigned)((scaled - (float)hi) * (float)(1u << 24));
-  }
-  __device__ __forceinline__ unsigned long long value() const { return ((unsigned long long)hi << 24) + lo; }
-};
-struct MassSum {
-  unsigned long long hi = 0, lo = 0;
-  __device__ __forceinline__ void add(Mass m) { hi += m.hi; lo += m.lo; }
-  __device__ __forceinline__ unsigned long long value() const { return (hi << 24) + lo; }
-};
-__device__ __forceinline__ unsigned long long mass_of(float s, float zmax) { return Mass(exp_of(s - zmax)).value(); }
+// The mass of a candidate, cut to 44 binary places: candidates come in no particular order, and sums of these do not depend on it.
+// (Sums over a row, which are made in one order, are sums of the exponentials as doubles: a third of the work.)
+__device__ __forceinline__ unsigned long long mass_of(float s, float zmax) {
+  return (unsigned long long)(exp_of(s - zmax) * (float)(1ull << FIX_PLACES));
+}
+constexpr double MASS_UNIT = 1.0 / (double)(1ull << FIX_PLACES);
+
+__device__ double block_sum_double(double v, double* red) {
+  for (int o = MS_WAVE / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
+  __syncthreads();
+  if ((threadIdx.x & (MS_WAVE - 1)) == 0) red[threadIdx.x / MS_WAVE] = v;
+  __syncthreads();
+  double s = 0.0;
+  for (int w = 0; w < WAVES; ++w) s += red[w];
+  return s;
+}
 
 __device__ unsigned long long block_sum_u64(unsigned long long v, unsigned long long* red) {
   for (int o = MS_WAVE / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
@@ -154,9 +155,9 @@ __device__ __forceinline__ unsigned largest_key(const RowWork& w, int n_chunks) 
   for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) best = max(best, (unsigned)__shfl_xor((int)best, o, MS_WAVE));
   return __builtin_amdgcn_readfirstlane(best);
 }
-__device__ __forceinline__ unsigned long long sum_of(const unsigned long long* chunks, int n_chunks) {
+__device__ __forceinline__ double sum_of(const double* chunks, int n_chunks) {
   const int lane = threadIdx.x & (MS_WAVE - 1);
-  unsigned long long v = lane < n_chunks ? chunks[lane] : 0ull;
+  double v = lane < n_chunks ? chunks[lane] : 0.0;
   for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
   return __shfl(v, 0, MS_WAVE);
 }
@@ -188,12 +189,12 @@ probabilities_max_kernel(const float* __restrict__ logits, size_t ld, int V, con
     if (threadIdx.x == 0) {
       for (int k = 1; k < WAVES; ++k) best = better(best, red_mi[k]);
       w.chunk_max[c] = __float_as_uint(best.v);
-      w.chunk_mass[c] = (unsigned)best.i;
+      w.chunk_first[c] = best.i;
     }
     return;
   }
   if (c == 0 && threadIdx.x == 0) { w.n_candidates = 0u; w.n_ties = 0u; w.bin = -1; w.bound = 0u; }
-  if (threadIdx.x == 0) { w.chunk_mass[c] = 0ull; w.chunk_above[c] = 0ull; }
+  if (threadIdx.x == 0) { w.chunk_mass[c] = 0.0; w.chunk_above[c] = 0.0; }
   if (a.use_p && !a.k && !a.all)
     for (int i = c * THREADS + threadIdx.x; i < BINS; i += n_chunks * THREADS) w.hist[i] = 0.f;
   unsigned best = 0;
@@ -216,12 +217,35 @@ probabilities_max_kernel(const float* __restrict__ logits, size_t ld, int V, con
   }
 }
 
+// A block's candidates, gathered here and handed over at once (an addition in memory for each was waited for by its wave).
+struct Candidates {
+  unsigned n, base, keys[MAX_CANDIDATES];
+  __device__ __forceinline__ void add(unsigned key) {
+    const unsigned at = atomicAdd(&n, 1u);
+    if (at < MAX_CANDIDATES) keys[at] = key;
+  }
+  __device__ void begin() {      // (the block does these two together)
+    if (threadIdx.x == 0) n = 0u;
+    __syncthreads();
+  }
+  __device__ void hand_over(RowWork& w) {
+    __syncthreads();
+    if (n == 0u) return;
+    if (threadIdx.x == 0) base = atomicAdd(&w.n_candidates, n);
+    __syncthreads();
+    const unsigned at = base + threadIdx.x;
+    if (threadIdx.x < n && at < MAX_CANDIDATES) w.candidates[at] = keys[threadIdx.x];
+  }
+};
+
 // ---- 2
 __global__ void __launch_bounds__(THREADS)
 probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
                              const int* __restrict__ top_k, const float* __restrict__ top_p, RowWork* __restrict__ work, int n_chunks) {
   __shared__ unsigned long long red[WAVES];
+  __shared__ double red_d[WAVES];
   __shared__ float hist[BINS];
+  __shared__ Candidates here;
   const int r = blockIdx.y, c = blockIdx.x;
   RowWork& w = work[r];
   const RowPlan a = plan_of(temperature, top_k, top_p, r, V, n_chunks);
@@ -232,10 +256,12 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
   const float zmax = key_value(largest_key(w, n_chunks));
   if (!finite(zmax)) return;      // no mass: the last kernel puts a one where the greedy choice stands
   if ((a.k || a.use_p) && a.all) {
+    here.begin();
     for_values(row, V, begin, end, [&](float v) {
       const float s = v * a.inv_t;
-      if (s == s) w.candidates[atomicAdd(&w.n_candidates, 1u)] = order_key(s);
+      if (s == s) here.add(order_key(s));
     });
+    here.hand_over(w);
     return;
   }
   if (a.k) {
@@ -274,16 +300,15 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
     const unsigned bound = n <= 4 * MS_WAVE ? kth(std::integral_constant<int, 4>{}) : n <= 8 * MS_WAVE ? kth(std::integral_constant<int, 8>{})
                                                                                     : kth(std::integral_constant<int, MAX_CHUNKS * WAVES * 4 / MS_WAVE>{});
     unsigned ties = 0;
+    here.begin();
     for_values(row, V, begin, end, [&](float v) {
       const float s = v * a.inv_t;
       if (!(s == s)) return;
       const unsigned key = order_key(s);
-      if (key > bound) {
-        const unsigned at = atomicAdd(&w.n_candidates, 1u);
-        if (at < MAX_CANDIDATES) w.candidates[at] = key;
-      }
+      if (key > bound) here.add(key);
       ties += key == bound;
     });
+    here.hand_over(w);
     const unsigned long long all = block_sum_u64(ties, red);
     if (threadIdx.x == 0) {
       if (all) atomicAdd(&w.n_ties, (unsigned)all);
@@ -291,45 +316,48 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
     }
     return;
   }
-  MassSum mine;
+  double mine = 0.0;
   if (!a.use_p) {
-    for_values(row, V, begin, end, [&](float v) { mine.add(Mass(exp_of(v * a.inv_t - zmax))); });
+    for_values(row, V, begin, end, [&](float v) { mine += (double)exp_of(v * a.inv_t - zmax); });
   } else {
     for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0.f;
     __syncthreads();
     for_values(row, V, begin, end, [&](float v) {
       const float s = v * a.inv_t, e = exp_of(s - zmax), x = (zmax - s) * BINS_A_UNIT;
-      mine.add(Mass(e));
+      mine += (double)e;
       if (x < (float)BINS) unsafeAtomicAdd(&hist[(int)x], e);
     });
     __syncthreads();
     for (int i = threadIdx.x; i < BINS; i += THREADS)
       if (hist[i] != 0.f) unsafeAtomicAdd(&w.hist[i], hist[i]);
   }
-  const unsigned long long mass = block_sum_u64(mine.value(), red);
-  if (threadIdx.x == 0) w.chunk_mass[c] = mass;
+  mine = block_sum_double(mine, red_d);
+  if (threadIdx.x == 0) w.chunk_mass[c] = mine;
 }
 
-__device__ __forceinline__ unsigned long long target_of(float p, unsigned long long total) {      // as the sampler has it
+// What the mass of the larger values must not have reached: top_p times the whole, and a unit of mass at least, so that the largest
+// value is always kept.
+__device__ __forceinline__ unsigned long long target_of(float p, unsigned long long total) {
   const unsigned long long target = (unsigned long long)((double)p * (double)total);
   return target > 0 ? target : 1ull;
 }
+__device__ __forceinline__ double target_of(float p, double total) { return fmax((double)p * total, MASS_UNIT); }
 
 // ---- 3
 __global__ void __launch_bounds__(THREADS)
 probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
                           const int* __restrict__ top_k, const float* __restrict__ top_p, RowWork* __restrict__ work, int n_chunks) {
-  __shared__ unsigned long long red[WAVES];
+  __shared__ double red[WAVES];
   __shared__ float wave_sum_sm[WAVES];
   __shared__ int found;
+  __shared__ Candidates here;
   const int r = blockIdx.y, c = blockIdx.x, lane = threadIdx.x & (MS_WAVE - 1), wave = threadIdx.x / MS_WAVE;
   RowWork& w = work[r];
   const RowPlan a = plan_of(temperature, top_k, top_p, r, V, n_chunks);
   if (a.greedy || a.k || !a.use_p || a.all) return;
   const float zmax = key_value(largest_key(w, n_chunks));
   if (!finite(zmax)) return;
-  const unsigned long long total = sum_of(w.chunk_mass, n_chunks);
-  const float target = (float)((double)target_of(a.p, total) / (double)(1ull << FIX_PLACES));
+  const float target = (float)((double)a.p * sum_of(w.chunk_mass, n_chunks));
   // the first bin at which the running mass reaches the target; a thread owns two bins
   const float h0 = w.hist[2 * threadIdx.x], h1 = w.hist[2 * threadIdx.x + 1];
   float run = h0 + h1;
@@ -351,26 +379,25 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   const float* row = logits + (size_t)r * ld;
   int begin, end;
   quad_range(row, V, n_chunks, c, &begin, &end);
-  unsigned long long above = 0;
+  double above = 0.0;
+  here.begin();
   for_values(row, V, begin, end, [&](float v) {
     const float s = v * a.inv_t;
-    if (s > high) {
-      above += mass_of(s, zmax);
-    } else if (s >= low) {
-      const unsigned at = atomicAdd(&w.n_candidates, 1u);
-      if (at < MAX_CANDIDATES) w.candidates[at] = order_key(s);
-    }
+    if (s > high) above += (double)exp_of(s - zmax);
+    else if (s >= low) here.add(order_key(s));
   });
-  above = block_sum_u64(above, red);
+  here.hand_over(w);
+  above = block_sum_double(above, red);
   if (threadIdx.x == 0) w.chunk_above[c] = above;
 }
 
-struct Kept { unsigned floor; unsigned long long mass; };
+struct Kept { unsigned floor; double mass; };
 
 // The floor by a radix descent of this block over the whole row, and the mass of what is kept.
 __device__ Kept descend(const float* __restrict__ row, int V, const RowPlan& a, float zmax, unsigned* lc, unsigned long long* lm) {
   const int quads = (lead_of(row) + V + 3) / 4, lane = threadIdx.x & (MS_WAVE - 1);
-  // the key at which the running count (or mass) from the top reaches `need`, among keys of at least `least`; with the mass upto it
+  unsigned long long total = 0;
+  // the key at which the running count (or mass) from the top reaches `need`, among keys of at least `least`; total: the mass upto it
   auto search = [&](bool by_mass, unsigned long long need, unsigned least) {
     unsigned digits = 0;
     unsigned long long above = 0, mass = 0;
@@ -403,12 +430,13 @@ __device__ Kept descend(const float* __restrict__ row, int V, const RowPlan& a, 
       above += by_mass ? f.mass_above : f.count_above;
       mass += f.mass_above + (level == 3 ? f.mass_in : 0ull);
     }
-    return Kept{digits, mass};
+    total = mass;
+    return digits;
   };
-  Kept k = search(false, a.k ? (unsigned long long)a.k : ~0ull >> 1, 0u);
-  if (!a.k) k.floor = 0u;
-  if (!a.use_p) return k;
-  return search(true, target_of(a.p, k.mass), k.floor);
+  unsigned floor = search(false, a.k ? (unsigned long long)a.k : ~0ull >> 1, 0u);
+  if (!a.k) floor = 0u;
+  if (a.use_p) floor = search(true, target_of(a.p, total), floor);
+  return Kept{floor, (double)total * MASS_UNIT};
 }
 
 // ---- 4
@@ -446,7 +474,7 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
   if (a.greedy) {
     const int lane = threadIdx.x & (MS_WAVE - 1);
     MaxIdx best = {-INFINITY, 0x7fffffff};
-    if (lane < n_chunks) best = MaxIdx{__uint_as_float(w.chunk_max[lane]), (int)w.chunk_mass[lane]};
+    if (lane < n_chunks) best = MaxIdx{__uint_as_float(w.chunk_max[lane]), w.chunk_first[lane]};
     for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) best = better(best, MaxIdx{__shfl_xor(best.v, o, MS_WAVE), __shfl_xor(best.i, o, MS_WAVE)});
     best.i = __shfl(best.i, 0, MS_WAVE);
     one = best.i == 0x7fffffff ? 0 : best.i;
@@ -463,56 +491,80 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
     return;
   }
 
-  Kept kept = {0u, 0ull};
+  Kept kept = {0u, 0.0};
   if (!a.k && !a.use_p) {
     kept.mass = sum_of(w.chunk_mass, n_chunks);
   } else {
+    // A candidate knows how many are larger, and their mass.  Top-k keeps it if these are fewer than k; top-p if what is larger has
+    // not reached the target.  Values equal to the bound are one candidate more, as often as they were counted.
     const int n = (int)w.n_candidates;
     bool known = n <= MAX_CANDIDATES && (a.all || (a.k ? a.groups > 0 : w.bin >= 0));
-    if (known) {
-      // a thread to a candidate; values equal to the bound are one more, as often as they were counted
-      const bool tied = a.k && !a.all;
-      const unsigned ties = tied ? w.n_ties : 0u;
-      const unsigned long long tie_mass = tied ? mass_of(key_value(w.bound), zmax) : 0ull;
-      unsigned mine = 0u;
-      unsigned long long mass = 0ull, above_all = 0ull;
+    const bool tied = a.k && !a.all, above_them = !a.k && !a.all;
+    const unsigned ties = tied ? w.n_ties : 0u, bound = w.bound;
+    const unsigned long long tie_mass = tied ? ties * mass_of(key_value(bound), zmax) : 0ull;
+    const bool ties_in_k = ties > 0 && n < a.k;
+    const double above = above_them ? sum_of(w.chunk_above, n_chunks) : 0.0, whole = above_them ? sum_of(w.chunk_mass, n_chunks) : 0.0;
+    unsigned mine = 0u;
+    unsigned long long mass = 0ull, larger = 0ull;
+    unsigned count = 0;
+    if (known && n <= MS_WAVE) {
+      // few enough for a wave: every wave of the block does it for itself
+      const int lane = threadIdx.x & (MS_WAVE - 1);
+      if (lane < n) {
+        mine = w.candidates[lane];
+        mass = mass_of(key_value(mine), zmax);
+      }
+      for (int j = 0; j < n; ++j) {
+        const unsigned key = __builtin_amdgcn_readlane(mine, j);
+        const unsigned hi = __builtin_amdgcn_readlane((unsigned)(mass >> 32), j), lo = __builtin_amdgcn_readlane((unsigned)mass, j);
+        const unsigned long long theirs = ((unsigned long long)hi << 32) | lo;
+        count += key > mine;
+        larger += key > mine ? theirs : 0ull;
+      }
+      const auto sum = [&](unsigned long long v) {
+        for (int o = MS_WAVE / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
+        return v;
+      };
+      bool in = lane < n && (!a.k || count < (unsigned)a.k), ties_in = ties_in_k;
+      unsigned long long kept_mass = sum(in ? mass : 0ull) + (ties_in ? tie_mass : 0ull);
+      if (a.use_p) {
+        const double target = target_of(a.p, above_them ? whole : (double)kept_mass * MASS_UNIT);
+        known = above < target && above + (double)kept_mass * MASS_UNIT >= target;      // (it falls among the candidates)
+        ties_in = ties_in && (double)(kept_mass - tie_mass) * MASS_UNIT < target;
+        in = in && above + (double)larger * MASS_UNIT < target;
+        kept_mass = sum(in ? mass : 0ull) + (ties_in ? tie_mass : 0ull);
+      }
+      unsigned floor = in ? mine : 0xffffffffu;
+      for (int o = MS_WAVE / 2; o > 0; o >>= 1) floor = min(floor, (unsigned)__shfl_xor((int)floor, o, MS_WAVE));
+      kept = Kept{ties_in ? min(floor, bound) : floor, above + (double)kept_mass * MASS_UNIT};
+    } else if (known) {
       if ((int)threadIdx.x < n) {
         mine = w.candidates[threadIdx.x];
         mass = mass_of(key_value(mine), zmax);
         keys[threadIdx.x] = mine;
         masses[threadIdx.x] = mass;
       }
-      if (!a.k && !a.all) above_all = sum_of(w.chunk_above, n_chunks);
       if (threadIdx.x == 0) floor_sm = 0xffffffffu;
       __syncthreads();
-      unsigned count = 0;
-      unsigned long long larger = above_all;
       if ((int)threadIdx.x < n)
         for (int j = 0; j < n; ++j)
           if (keys[j] > mine) { ++count; larger += masses[j]; }
-      // what top-k keeps (the bound's values are kept if fewer than k are larger)
-      const bool in_k = (int)threadIdx.x < n && (!a.k || count < (unsigned)a.k);
-      const bool ties_in_k = ties > 0 && (unsigned)n < (unsigned)a.k;
-      unsigned long long total = above_all + block_sum_u64(in_k ? mass : 0ull, red) + (ties_in_k ? ties * tie_mass : 0ull);
-      bool in = in_k, ties_in = ties_in_k;
+      bool in = (int)threadIdx.x < n && (!a.k || count < (unsigned)a.k), ties_in = ties_in_k;
+      unsigned long long kept_mass = block_sum_u64(in ? mass : 0ull, red) + (ties_in ? tie_mass : 0ull);
       if (a.use_p) {
-        unsigned long long whole = total;
-        if (!a.k && !a.all) whole = sum_of(w.chunk_mass, n_chunks);
-        const unsigned long long target = target_of(a.p, whole);
-        known = above_all < target && total >= target;      // (it falls among the candidates)
-        in = in_k && larger < target;
-        const unsigned long long all_in = block_sum_u64(in_k ? mass : 0ull, red);
-        ties_in = ties_in_k && all_in < target;
-        total = above_all + block_sum_u64(in ? mass : 0ull, red) + (ties_in ? ties * tie_mass : 0ull);
+        const double target = target_of(a.p, above_them ? whole : (double)kept_mass * MASS_UNIT);
+        known = above < target && above + (double)kept_mass * MASS_UNIT >= target;
+        ties_in = ties_in && (double)(kept_mass - tie_mass) * MASS_UNIT < target;
+        in = in && above + (double)larger * MASS_UNIT < target;
+        kept_mass = block_sum_u64(in ? mass : 0ull, red) + (ties_in ? tie_mass : 0ull);
       }
       if (in) atomicMin(&floor_sm, mine);
-      if (ties_in && threadIdx.x == 0) atomicMin(&floor_sm, w.bound);
       __syncthreads();
-      kept = Kept{floor_sm, total};
+      kept = Kept{ties_in ? min(floor_sm, bound) : floor_sm, above + (double)kept_mass * MASS_UNIT};
     }
     if (!known) kept = descend(row, V, a, zmax, keys, masses);
   }
-  const float inv = (float)((double)(1ull << FIX_PLACES) / (double)kept.mass), floor = kept.floor ? key_value(kept.floor) : -INFINITY;
+  const float inv = (float)(1.0 / kept.mass), floor = kept.floor ? key_value(kept.floor) : -INFINITY;
   for_quads(row, V, begin, end, [&](int i, const float4& v) {
     auto value = [&](float x) {
       const float s = x * a.inv_t;

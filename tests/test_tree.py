@@ -760,6 +760,50 @@ def test_the_step_replays_from_a_graph():
     assert results[0] != results[1] or results[1] != results[2]
 
 
+@gpu
+def test_the_sampler_and_the_pools_reach_them():
+    """``Sampler.probabilities`` and ``verify`` against the operators with the same settings; ``CachePools.keep_tokens`` moves the
+    entries of every group."""
+    from llm_infrence_engine_amd.cache.manager import CacheLayout
+    from llm_infrence_engine_amd.cache.pools import CachePools
+    from llm_infrence_engine_amd.parts.base import CacheNeed, PageTensor, Runtime
+    from llm_infrence_engine_amd.sampling.sampler import Sampler
+
+    g = torch.Generator().manual_seed(5)
+    rows = [SimpleNamespace(temperature=t, top_k=k, top_p=p) for t, k, p in ((0.8, 20, 0.9), (0.0, 5, 0.5), (1.2, 0, 1.0), (0.7, 0, 0.8))]
+    logits = 2 * torch.randn(4, 700, generator=g)
+    sampler = Sampler(torch.device(DEV))
+    got = sampler.probabilities(logits.to(DEV), rows).cpu().double()
+    want = plain_probabilities(logits, torch.tensor([r.temperature for r in rows]), ints([r.top_k for r in rows], "cpu"), torch.tensor([r.top_p for r in rows]))
+    assert ((got - want).abs() <= 2.8e-6 * want + 1e-30).all()
+    greedy = [SimpleNamespace(temperature=0.0, top_k=0, top_p=1.0)] * 4
+    assert torch.equal(sampler.probabilities(logits.to(DEV), greedy).argmax(1).cpu(), logits.argmax(1))
+    with pytest.raises(ValueError):
+        sampler.probabilities(logits.to(DEV), rows[:3])
+    made = make_drafts([5, 9], 300, 2)
+    paths, drawn = plain_verify(*made, 9)
+    p, q, tokens, parents, starts, u = made
+    nodes, counts, out = sampler.verify(p.to(DEV), q.to(DEV), ints(tokens), ints(parents), ints(starts), u.to(DEV), 9)
+    assert counts.tolist() == [len(x) for x in paths] and out.tolist() == drawn and [n[:c] for n, c in zip(nodes.tolist(), counts.tolist())] == paths
+
+    rt = Runtime(device=torch.device(DEV), dtype=BF16)
+    wide = CacheNeed((PageTensor("k", 2, 64), PageTensor("v", 2, 64, transpose_at=16)), None)
+    narrow = CacheNeed((PageTensor("k", 1, 32), PageTensor("v", 1, 32, transpose_at=16)), 40)
+    pools = CachePools(CacheLayout([(wide, None, None), (narrow, None, None), (wide, None, None)]), 16, 8, 2, rt, 4)
+    for table, row in zip(pools.tables, ([3, 1, 2, 0], [5, 0, 7, 4])):
+        table[1] = ints(row)
+    before = []
+    for pages in pools.pages:
+        for t in pages.values():
+            t.normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+        before.append({n: t.cpu().clone() for n, t in pages.items()})
+    pools.keep_tokens(ints([30]), ints([[0, 2, 5, -1]]), ints([3]), ints([1]))
+    for pages, flips, table, old in zip(pools.pages, pools.transposed, pools.tables, before):
+        assert flips["v"] and not flips["k"]
+        for n, t in pages.items():
+            assert torch.equal(t.cpu(), plain_keep(old[n], flips[n], table.cpu(), [1], [30], [[0, 2, 5]], [3]))
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU needed)
 @pytest.fixture
 def host(monkeypatch):
@@ -886,3 +930,13 @@ def test_tree_attention_refuses(host):
     refused(host, lambda: args(context_lens=torch.zeros(2)))
     args()
     assert host == ["ms_tree_attention_generic"]
+
+
+def test_pools_that_cannot_drop_tokens_refuse(host):
+    from llm_infrence_engine_amd.cache.pools import CachePools
+
+    z = torch.zeros(1, dtype=torch.int32)
+    for state, strides in (({0: ()}, [1]), ({}, [1, 4])):
+        pools = CachePools.__new__(CachePools)
+        pools.state, pools.layout = state, SimpleNamespace(group_keys=[SimpleNamespace(stride=s) for s in strides])
+        refused(host, lambda: pools.keep_tokens(z, z.view(1, 1), z, z))
