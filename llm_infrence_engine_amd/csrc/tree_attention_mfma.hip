@@ -227,7 +227,7 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
       }
     }
     if (!works || t >= t_end) continue;      // the same for the whole wave
-#pragma unroll 1
+#pragma unroll
     for (int unit = 0; unit < KEYS / 32; unit += UNITS) {
     const int base = t * KEYS + unit * 32;
     const bf16* st = lds + (kg * 2 + stage) * STAGE + unit * 2 * CHUNK;
