@@ -11,6 +11,10 @@
 // where row r of the u-th score product of a unit of 32 keys is its key 8 (r / 4) + 4 u + r % 4, so that a lane (quarter kq)
 // holds the scores of the keys 8 kq .. + 7 and needs one 16-byte read of a value's row.  Keys from before the step are visible
 // to every column; only units that reach into the step's own entries (the last ones) look at the mask.
+// Rounding: the weights e^(s - ref) meet the values as bfloat16, since that is what the product takes; each is off by 2^-8 of
+// itself at most, and the sum that divides is of the rounded ones.  Scores, exponentials, sums and results up to the last
+// rounding are float.  Against 64 bits the result is off by 0.0018 to 0.0023 of its norm, of which the rounding of the result
+// itself makes 0.0017 (4 trees of up to 63 behind 16,011 keys; 32 trees of up to 13 behind some 4,000).
 // The keys of a request are shared out over n_splits blocks, which leave unnormalised float results that a second kernel
 // adds up: with few columns there is one (request, head) tile for a handful of CUs, and a step waits for the longest chain.
 #include "attention_tiles.h"
@@ -199,9 +203,8 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
   }
   const int v_row = CHUNKS * CHUNK + (kq >> 1) * CHUNK + col16 * 16 + (((kq & 1) ^ (col16 >> 3)) * 8);     // .. and of 16 dims' values
 
-  // The queries and masks have arrived: said here, by a use that nothing moves past the loop.  Otherwise the compiler waits for
-  // them, and with them for the tile that has just been asked for, before the first product of every turn (5,376 keys on one
-  // block a CU, 64 columns of 128 dims: 1.05 us a tile).
+  // The queries and masks have arrived: said here, by a use that nothing moves past the loop.  Otherwise the compiler may wait for
+  // them, and with them for the tile that has just been asked for, before the first product of every turn.
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -232,9 +235,9 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
     const int base = t * KEYS + unit * 32;
     const bf16* st = lds + (kg * 2 + stage) * STAGE + unit * 2 * CHUNK;
 
-    // scores: s[n][u][t] holds keys base + n*32 + kq*8 + u*4 + (0..3) of column t*16 + col16.  The units of a tile go through
-    // every stage together: a wave's products wait for each other (0.9 us a unit of 32 keys where a CU has one block, 0.45 of
-    // them products), and those of another unit can run meanwhile.
+    // scores: s[n][u][t] holds keys base + n*32 + kq*8 + u*4 + (0..3) of column t*16 + col16.  With one tile of columns the units
+    // go through every stage together, so that products of one run while the other waits for its own; with two there are no
+    // registers for it.
     f32x4 s[UNITS][2][NT];
 #pragma unroll
     for (int n = 0; n < UNITS; ++n)
@@ -707,6 +710,15 @@ inline long long column_tiles(int n_requests, int n_tokens, int max_q_len, int r
   return std::min((long long)n_tokens * rep / cols + n_requests, ((long long)max_q_len * rep + cols - 1) / cols * n_requests);
 }
 
+// Allows a kernel more LDS than the default 64 KB, once on every device it runs on (`raised`: the kernel's own flags).
+constexpr int MAX_DEVICES = 64;
+inline bool raise_lds(const void* kernel, size_t bytes, bool* raised) {
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= MAX_DEVICES) return false;
+  if (!raised[dev]) raised[dev] = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
+  return raised[dev];
+}
+
 inline int page_shift_of(int page_size) {   // log2 of a power of two, else -1
   return page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size);
 }
@@ -714,13 +726,8 @@ inline int page_shift_of(int page_size) {   // log2 of a power of two, else -1
 template <int D, int WC, int KG, int NT>
 int launch(const Call& a) {
   typedef Shape<D, WC, KG, NT> S;
-  static bool raised = false;   // once per instantiation: allow more LDS than the default 64 KB
-  if (!raised) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_attention_mfma_kernel<D, WC, KG, NT>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::LDS) != hipSuccess)
-      return MS_LAUNCH_FAILED;
-    raised = true;
-  }
+  static bool raised[MAX_DEVICES] = {};
+  if (!raise_lds(reinterpret_cast<const void*>(&tree_attention_mfma_kernel<D, WC, KG, NT>), S::LDS, raised)) return MS_LAUNCH_FAILED;
   const int rep = a.nh / a.nkv;
   const bool one = (long long)a.max_q_len * rep <= S::COLS;
   const long long tiles = one ? a.n_requests : column_tiles(a.n_requests, a.n_tokens, a.max_q_len, rep, S::COLS);
@@ -737,22 +744,24 @@ int launch(const Call& a) {
 }
 
 // Kinds of block: WC waves over columns, KG groups over keys (at 32 and 64 dims F times as many), NT tiles of 16 columns a wave.
-// A block's time is a chain of turns (KG tiles of keys): 5.5 us before and after it, `alone` us a turn with one block on a CU,
-// `pair` where there are two (0: its LDS leaves room for one).
+// A block's time is a chain of turns (KG tiles of keys): 2.1 us around them, `alone` us a turn with one block on a CU, `pair`
+// where there are two (0: its LDS leaves room for one).
 struct Kind { int wc, kg, nt; double alone, pair; };
-constexpr Kind KINDS[2][4] = {{{1, 8, 1, 0.9, 0.0}, {2, 4, 1, 0.7, 0.9}, {4, 2, 1, 0.9, 1.2}, {4, 1, 2, 1.2, 1.5}},     // 32, 64 dims
-                              {{1, 4, 1, 0.6, 0.0}, {2, 2, 1, 0.7, 0.8}, {4, 1, 1, 1.15, 1.35}, {4, 1, 2, 1.7, 2.1}}};  // 128 dims
+constexpr Kind KINDS[2][4] = {{{1, 8, 1, 0.75, 0.0}, {2, 4, 1, 0.37, 1.02}, {4, 2, 1, 0.73, 1.37}, {4, 1, 2, 0.93, 1.19}},     // 32, 64 dims
+                              {{1, 4, 1, 1.22, 0.0}, {2, 2, 1, 0.64, 0.89}, {4, 1, 1, 1.13, 1.12}, {4, 1, 2, 1.62, 1.83}}};  // 128 dims
 
 }  // namespace
 
 // kind * 65536 + how many times 64 keys a block takes, for a step of these sizes (all bounds); -1: sizes this kernel does not
 // take.  Narrow kinds share a small step out over the chip, and every block's chain is short; wide ones read the keys less
-// often.  The choice is the least of a model: the chains, as often as all blocks take the chip's room, or the keys at 9 TB/s
-// (what all tiles of columns drew together, from L2s and memory), whichever is longer, and the second kernel (2.8 us, the
-// parts written and read at 3 TB/s).  us measured, the model's choice against the fastest of kinds and shares: 8 tokens of
-// 14 heads of 64 on 2 behind 192 keys 6.3, 6.3 (63 columns a block: 7.9); 32 x 8 behind 700 9.2, 9.2 (12.2); 32 tokens behind
-// 8,000 14.3, 14.3 (21.1 of 128 columns); 28 heads of 128 on 4: 8 x 16 behind 2,000 23.9, 21.8; 32 x 8 behind 1,000 22.8, 22.8
-// (16 columns: 33.7); 40 on 8: 2 x 16 behind 4,000 22.4, 19.9, 4 x 63 behind 16,011 107, 107 (16 columns: 311).
+// often.  The choice is the least of a model: a launch (4.3 us), then the chains, as often as all blocks take the chip's room, or
+// the keys at 13.5 TB/s (what all tiles of columns drew together, from L2s and memory), whichever is longer, and the second kernel
+// (3.1 us, the parts written and read at 4.4 TB/s).  Its numbers are fitted to the times of all kinds and shares at 44 steps of 64
+// and 128 dims (1 to 64 requests of 1 to 63 tokens behind 64 to 16,011 keys); there its choice takes 1.7% longer than the fastest on
+// average, 15% at most.  us measured, the choice against the fastest and the slowest kind with its best share: 8 tokens of 14
+// heads of 64 on 2 behind 192 keys 6.7, 6.7 (128 columns a block: 9.2); 28 heads of 128 on 4: 8 x 16 behind 2,000 19.0, 19.0
+// (16 columns: 25.1), 32 x 8 behind 1,000 22.5, 20.5 (16 columns: 31.3); 40 on 8: 2 x 16 behind 4,000 19.2, 18.9 (128 columns: 21.1),
+// 4 x 63 behind 16,011 101, 101 (16 columns: 274).
 extern "C" int ms_tree_attention_mfma_plan(int n_requests, int n_tokens, int max_q_len, int max_context_len, int num_heads,
                                            int num_kv_heads, int head_dim, int page_size) {
   if ((head_dim != 32 && head_dim != 64 && head_dim != 128) || page_size <= 0 || page_size % 16) return -1;
@@ -769,15 +778,15 @@ extern "C" int ms_tree_attention_mfma_plan(int n_requests, int n_tokens, int max
     const int width = k.wc * k.nt * 16, turn = (k.wc == 4 ? 64 : 32) * k.kg;
     // a request ends in half a tile on average, unless one tile is all it has
     const double tiles = ((long long)max_q_len * rep <= width ? (double)n_requests : cols / width + 0.5 * n_requests) * num_kv_heads;
-    const double draws = tiles * context * head_dim * 4 / 9e6;
+    const double draws = tiles * context * head_dim * 4 / 13.5e6;
     for (const int n : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128}) {
       const long long share = ((context + n - 1) / n + turn - 1) / turn * turn, turns = share / turn, splits = (context + share - 1) / share;
       if (splits > MAX_SPLITS) continue;
       const double blocks = tiles * splits;
       const bool pairs = k.pair > 0.0 && blocks > cus;
       const double rounds = std::max(1.0, blocks / (pairs ? 2.0 * cus : cus));
-      double us = 5.5 + std::max(turns * (pairs ? k.pair : k.alone) * rounds, draws);
-      if (splits > 1) us += 2.8 + (double)n_tokens * num_heads * splits * (head_dim + 2) * 8 / 3e6;
+      double us = 4.3 + std::max((turns * (pairs ? k.pair : k.alone) + 2.1) * rounds, draws);
+      if (splits > 1) us += 3.1 + (double)n_tokens * num_heads * splits * (head_dim + 2) * 8 / 4.4e6;
       if (choice < 0 || us < best) { best = us; choice = kind * 65536 + (int)(share / 64); }
       if (n > 1 && turns == 1) break;
     }
@@ -846,13 +855,8 @@ extern "C" int ms_tree_attention_f32(const float* q, long long q_stride, const f
   auto go = [&](auto dims, auto nt) {
     constexpr int D = decltype(dims)::value, NT = decltype(nt)::value;
     constexpr int lds = F32_WAVES * (D / 16) * NT * MS_WAVE * (int)sizeof(f32x4);
-    static bool raised = false;   // once per instantiation: allow more LDS than the default 64 KB
-    if (!raised) {
-      if (hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_attention_f32_kernel<D, NT>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
-        return (int)MS_LAUNCH_FAILED;
-      raised = true;
-    }
+    static bool raised[MAX_DEVICES] = {};
+    if (!raise_lds(reinterpret_cast<const void*>(&tree_attention_f32_kernel<D, NT>), lds, raised)) return (int)MS_LAUNCH_FAILED;
     const bool one = (long long)max_q_len * rep <= NT * 16;
     const long long tiles = one ? n_requests : column_tiles(n_requests, n_tokens, max_q_len, rep, NT * 16);
     if (tiles > 65535) return (int)MS_UNSUPPORTED;
