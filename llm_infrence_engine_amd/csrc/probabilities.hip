@@ -9,13 +9,14 @@
 //     it (50 of 384 groups: 54 expected): these are collected as candidates, those equal to it counted
 //     top-p alone: every chunk's mass, and a histogram of masses by the distance from the maximum (1/128 wide, 2,048 of them), in
 //     float: its sums depend on the order, so it only says where to look
-//   3 top-p alone: the values of the histogram's bin in which the target falls, and of its neighbours, are the candidates;
-//     the mass above them is summed up exactly
-//   4 a thread to a candidate: count and mass of the larger ones say whether it is kept, the least kept one is the floor; then
-//     every block writes its chunk
+//   3 top-p alone: the values of the histogram's bin in which the target falls, with a neighbour's where it falls that near its
+//     edge, are the candidates; the mass above them is summed up anew, in double
+//   4 a thread to a candidate: count and mass of the larger ones say whether it is kept, the least kept one is the floor (from many
+//     candidates a radix descent over their keys finds it); then every block writes its chunk
 // What the candidates cannot decide (more than MAX_CANDIDATES of them, a k beyond half the groups, a target outside the
 // candidates' masses) every block of the row finds by itself with a radix descent over the whole row: right for any input, and
-// slow (a row of 151,936: about 100 us).
+// slow (a row of 151,936: 110 us for a k of half of them, 190 for top-p 0.5 of normal logits at a temperature of 3, 360 where all are
+// alike; 28 to 45 otherwise).
 #include "sampling.h"
 #include "api.h"
 #include <algorithm>
@@ -31,6 +32,7 @@ constexpr int MAX_CHUNKS = 32, WAVES = THREADS / MS_WAVE;
 constexpr int MAX_CANDIDATES = THREADS;
 constexpr int BINS = 2048;
 constexpr float BINS_A_UNIT = 128.f;
+constexpr float NEAR_EDGE = 1.0f / 32768.f;      // of the whole mass; sums of up to 152,064 floats in any order are closer to their own
 
 struct RowWork {                       // one per row, in the workspace the caller brings
   unsigned chunk_max[MAX_CHUNKS];      // key of the largest scaled logit of every chunk (no temperature: the largest itself)
@@ -338,8 +340,8 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
 // What the mass of the larger values must not have reached: top_p times the whole, and a unit of mass at least, so that the largest
 // value is always kept.
 __device__ __forceinline__ unsigned long long target_of(float p, unsigned long long total) {
-  const unsigned long long target = (unsigned long long)((double)p * (double)total);
-  return target > 0 ? target : 1ull;
+  const double target = (double)p * (double)total;
+  return target >= 1.0 ? (unsigned long long)target : 1ull;
 }
 __device__ __forceinline__ double target_of(float p, double total) { return fmax((double)p * total, MASS_UNIT); }
 
@@ -349,7 +351,7 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
                           const int* __restrict__ top_k, const float* __restrict__ top_p, RowWork* __restrict__ work, int n_chunks) {
   __shared__ double red[WAVES];
   __shared__ float wave_sum_sm[WAVES];
-  __shared__ int found;
+  __shared__ int found, up, down;      // the target's bin; those before and behind it that count too
   __shared__ Candidates here;
   const int r = blockIdx.y, c = blockIdx.x, lane = threadIdx.x & (MS_WAVE - 1), wave = threadIdx.x / MS_WAVE;
   RowWork& w = work[r];
@@ -357,7 +359,8 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   if (a.greedy || a.k || !a.use_p || a.all) return;
   const float zmax = key_value(largest_key(w, n_chunks));
   if (!finite(zmax)) return;
-  const float target = (float)((double)a.p * sum_of(w.chunk_mass, n_chunks));
+  const double whole = sum_of(w.chunk_mass, n_chunks);
+  const float target = (float)((double)a.p * whole), near = (float)whole * NEAR_EDGE;
   // the first bin at which the running mass reaches the target; a thread owns two bins
   const float h0 = w.hist[2 * threadIdx.x], h1 = w.hist[2 * threadIdx.x + 1];
   float run = h0 + h1;
@@ -373,8 +376,13 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   __syncthreads();
   // (sums of floats may fall short of a target that is nearly everything: the last bin that has any would be no surer)
   if (found >= BINS) return;
-  // its bin and the one on either side, as values
-  const float high = zmax - (float)(found - 1) * (1.0f / BINS_A_UNIT), low = zmax - (float)(found + 2) * (1.0f / BINS_A_UNIT);
+  if (found >> 1 == (int)threadIdx.x) {
+    const float upto = found & 1 ? run : run - h1, from = upto - (found & 1 ? h1 : h0);
+    up = target - from < near;
+    down = upto - target < near;
+  }
+  __syncthreads();
+  const float high = zmax - (float)(found - up) * (1.0f / BINS_A_UNIT), low = zmax - (float)(found + 1 + down) * (1.0f / BINS_A_UNIT);
   if (c == 0 && threadIdx.x == 0) w.bin = found;
   const float* row = logits + (size_t)r * ld;
   int begin, end;
@@ -393,9 +401,12 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
 
 struct Kept { unsigned floor; double mass; };
 
-// The floor by a radix descent of this block over the whole row, and the mass of what is kept.
-__device__ Kept descend(const float* __restrict__ row, int V, const RowPlan& a, float zmax, unsigned* lc, unsigned long long* lm) {
-  const int quads = (lead_of(row) + V + 3) / 4, lane = threadIdx.x & (MS_WAVE - 1);
+// The floor among what `each` hands to its function, scaled logits in any order (NaN: nobody), and the mass of what is kept: a radix
+// descent of the block over their keys.  `need`, from the mass that top-k keeps, is what the larger values' must not have reached.
+template <typename Each, typename Need>
+__device__ __forceinline__ Kept descend(const Each& each, int k, bool use_p, const Need& need_of, float zmax, unsigned* lc,
+                                        unsigned long long* lm, unsigned long long* red) {
+  const int lane = threadIdx.x & (MS_WAVE - 1);
   unsigned long long total = 0;
   // the key at which the running count (or mass) from the top reaches `need`, among keys of at least `least`; total: the mass upto it
   auto search = [&](bool by_mass, unsigned long long need, unsigned least) {
@@ -406,8 +417,7 @@ __device__ Kept descend(const float* __restrict__ row, int V, const RowPlan& a, 
       __syncthreads();
       for (int i = threadIdx.x; i < bins; i += THREADS) { lc[i] = 0u; lm[i] = 0ull; }
       __syncthreads();
-      for_values(row, V, 0, quads, [&](float v) {
-        const float s = v * a.inv_t;
+      each([&](float s) {
         const unsigned key = order_key(s);
         const bool in = s == s && key >= least && (level == 1 || (key >> (shift + (level == 2 ? 11 : 10))) == digits);
         const int bin = (int)((key >> shift) & (unsigned)(bins - 1));
@@ -433,9 +443,19 @@ __device__ Kept descend(const float* __restrict__ row, int V, const RowPlan& a, 
     total = mass;
     return digits;
   };
-  unsigned floor = search(false, a.k ? (unsigned long long)a.k : ~0ull >> 1, 0u);
-  if (!a.k) floor = 0u;
-  if (a.use_p) floor = search(true, target_of(a.p, total), floor);
+  unsigned floor = 0u;
+  if (k) {
+    floor = search(false, (unsigned long long)k, 0u);
+  } else {
+    unsigned long long mine = 0ull;
+    each([&](float s) { mine += s == s ? mass_of(s, zmax) : 0ull; });
+    total = block_sum_u64(mine, red);
+  }
+  if (use_p) {
+    const unsigned long long need = need_of(total);
+    if (need == 0ull || need > total) return Kept{0u, 0.0};      // (it does not fall among them)
+    floor = search(true, need, floor);
+  }
   return Kept{floor, (double)total * MASS_UNIT};
 }
 
@@ -537,6 +557,17 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
       unsigned floor = in ? mine : 0xffffffffu;
       for (int o = MS_WAVE / 2; o > 0; o >>= 1) floor = min(floor, (unsigned)__shfl_xor((int)floor, o, MS_WAVE));
       kept = Kept{ties_in ? min(floor, bound) : floor, above + (double)kept_mass * MASS_UNIT};
+    } else if (known && !tied) {
+      // many, and each of them itself: the descent over them (one row of 151,936 normal logits, top-p 0.9 at temperatures 0.7 and 3:
+      // 41 and 45 us, compared with each other 58 and 100)
+      const float s = (int)threadIdx.x < n ? key_value(w.candidates[threadIdx.x]) : NAN;
+      kept = descend([&](auto f) { f(s); }, a.k, a.use_p, [&](unsigned long long total) -> unsigned long long {
+        if (!above_them) return target_of(a.p, total);
+        const double need = ceil((target_of(a.p, whole) - above) / MASS_UNIT);
+        return need >= 1.0 && need <= (double)total ? (unsigned long long)need : 0ull;
+      }, zmax, keys, masses, red);
+      known = kept.mass > 0.0;
+      kept.mass += above;
     } else if (known) {
       if ((int)threadIdx.x < n) {
         mine = w.candidates[threadIdx.x];
@@ -552,17 +583,20 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
       bool in = (int)threadIdx.x < n && (!a.k || count < (unsigned)a.k), ties_in = ties_in_k;
       unsigned long long kept_mass = block_sum_u64(in ? mass : 0ull, red) + (ties_in ? tie_mass : 0ull);
       if (a.use_p) {
-        const double target = target_of(a.p, above_them ? whole : (double)kept_mass * MASS_UNIT);
-        known = above < target && above + (double)kept_mass * MASS_UNIT >= target;
+        const double target = target_of(a.p, (double)kept_mass * MASS_UNIT);
         ties_in = ties_in && (double)(kept_mass - tie_mass) * MASS_UNIT < target;
-        in = in && above + (double)larger * MASS_UNIT < target;
+        in = in && (double)larger * MASS_UNIT < target;
         kept_mass = block_sum_u64(in ? mass : 0ull, red) + (ties_in ? tie_mass : 0ull);
       }
       if (in) atomicMin(&floor_sm, mine);
       __syncthreads();
-      kept = Kept{ties_in ? min(floor_sm, bound) : floor_sm, above + (double)kept_mass * MASS_UNIT};
+      kept = Kept{ties_in ? min(floor_sm, bound) : floor_sm, (double)kept_mass * MASS_UNIT};
     }
-    if (!known) kept = descend(row, V, a, zmax, keys, masses);
+    if (!known) {
+      const int quads = (lead_of(row) + V + 3) / 4;
+      kept = descend([&](auto f) { for_values(row, V, 0, quads, [&](float v) { f(v * a.inv_t); }); }, a.k, a.use_p,
+                     [&](unsigned long long total) { return target_of(a.p, total); }, zmax, keys, masses, red);
+    }
   }
   const float inv = (float)(1.0 / kept.mass), floor = kept.floor ? key_value(kept.floor) : -INFINITY;
   for_quads(row, V, begin, end, [&](int i, const float4& v) {
