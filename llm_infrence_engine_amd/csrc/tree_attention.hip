@@ -8,7 +8,7 @@
 // A token that sees nothing gets zeros.  What is not visible cannot reach a result: such a score is replaced, never
 // added to, and such a value is not multiplied (a NaN times a weight of zero would be one).
 // Scores, maximum, exponentials, their sum and the weighted sum of values are float.
-// This is the kernel of the 32-bit path and of sizes that csrc/tree_attention_mfma.hip does not take: a block owns one
+// This is the kernel of the sizes and layouts that csrc/tree_attention_mfma.hip does not take: a block owns one
 // (token, query head), its waves take blocks of 64 keys in turn (a lane reads its own key's row, then every lane its own
 // entries of one row of values after another) and are merged through LDS in order.
 #include "common.h"
@@ -30,6 +30,7 @@ tree_attention_kernel(const T* __restrict__ q, size_t q_stride, const T* __restr
   if (n_live_tokens && n >= *n_live_tokens) return;      // a token that pads a captured batch
   const int r = token_req[n], kvh = h / (nh / nkv);
   const int q0 = q_start[r], qlen = q_start[r + 1] - q0, context = context_lens[r], before = context - qlen;
+  if (n < q0 || n >= q0 + qlen) return;                  // (nor is one without a count of live ones)
   const int* table = block_table + (size_t)(table_rows ? table_rows[r] : r) * table_stride;
   const unsigned* bits = tree + (size_t)n * words;
   for (int i = threadIdx.x; i < d; i += WAVES * MS_WAVE) qs[i] = to_float(q[(size_t)n * q_stride + (size_t)h * d + i]) * scale;

@@ -1578,6 +1578,8 @@ def tree_attention_mfma(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     N, R = q.shape[0], context_lens.shape[0]
     if N == 0 or R == 0:
         return out
+    if max_context_len < 1 or max_context_len > block_table.shape[1] * page_size:
+        raise ValueError(f"max_context_len {max_context_len} does not fit a table of {block_table.shape[1]} pages of {page_size}")
     if small:
         plan = _get("ms_tree_attention_mfma_plan")(R, N, max_q_len, max_context_len, num_heads, nkv, d, page_size)
         kind, share = plan >> 16, (plan & 0xFFFF) * 64
@@ -1747,6 +1749,8 @@ def keep_tokens(pages, transposed, block_table: torch.Tensor, first: torch.Tenso
         elif sizes != (L, P, page_size):
             raise ValueError("the page tensors of a call have the same layers, pages and page size")
         record += _KEPT_TENSOR.pack(t.data_ptr(), heads, width, bool(flip), 0)
+    if len({t.data_ptr() for t in pages}) != n:
+        raise ValueError("a page tensor stands in the call twice")
     if R == 0 or depth == 0 or 0 in pages[0].shape:
         return
     if R > 65535:

@@ -249,6 +249,36 @@ def test_tree_attention_of_a_padded_batch(dtype):
     assert (out[N:] == 3.0).all()
 
 
+@gpu
+@pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (8, 2, 128), (4, 2, 32)])
+@pytest.mark.parametrize("kind", range(4))
+def test_tree_attention_of_every_kind_of_block(monkeypatch, nh, nkv, d, kind):
+    """Whatever kind of block and share of the keys a step's sizes ask for: 64 to 4,096 keys a block, some blocks without any."""
+    get = ops._get
+    for share in (64, 192, 448, 4096):
+        monkeypatch.setattr(ops, "_get", lambda name: (lambda *a: kind * 65536 + share // 64) if name == "ms_tree_attention_mfma_plan" else get(name))
+        s = make_step(BF16, nh, nkv, d, 16, [12, 0, 37, 1], [1301, 0, 75, 640], seed=7)
+        ops.tree_attention(s.q, s.kv, s.ctx, s.tree, s.out, s.nh, s.scale)
+        close_enough(s)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 48])
+def test_tree_attention_of_tokens_that_are_nobodys(dtype, d):
+    """Tokens behind the last request's stay as they are without a count of live ones too."""
+    s = make_step(dtype, 8, 2, d, 16, [5, 7], [40, 90], seed=9)
+    N = 12
+    pad, out = torch.zeros(15, 8 * d, dtype=dtype, device=DEV), torch.full((15, 8 * d), 3.0, device=DEV).to(dtype)
+    pad[:N] = s.q
+    tree = torch.full((15, 1), -1, dtype=torch.int32, device=DEV)
+    tree[:N] = s.tree
+    s.ctx.token_req = torch.cat([s.ctx.token_req, ints([0, 1, 1])])
+    ops.tree_attention(pad, s.kv, s.ctx, tree, out, 8, s.scale)
+    close_enough(s, out[:N])
+    assert (out[N:] == 3.0).all()
+
+
 # ------------------------------------------------------------------------------------------------ probabilities
 def plain_probabilities(logits, T, top_k, top_p):
     """float64, row by row; the scaled logits are floats, as the sampler has them."""
@@ -330,6 +360,57 @@ def test_probabilities_of_mixed_rows():
     check_probabilities(logits, T, None, None)
     check_probabilities(logits, None, None, None)
     check_probabilities(logits[:1].repeat(300, 1)[:, :77].contiguous(), torch.full((300,), 0.6), ints([9] * 300, "cpu"), None)
+
+
+@gpu
+@pytest.mark.parametrize("V", [2500, 40001, 151936])
+def test_probabilities_that_no_few_candidates_decide(V):
+    """Rows so flat, a k so large or a mass so near its whole that the kept values' edge lies among thousands; rows with two values
+    only; the same answer every time."""
+    g = torch.Generator().manual_seed(V)
+    logits = torch.randn(6, V, generator=g)
+    logits[0] *= 1e-3
+    logits[1] = 0.0
+    logits[2] = (torch.rand(V, generator=g) < 0.5).float()
+    logits[3, V // 2:] -= 60.0
+    T, k, p = torch.full((6,), 1.0), ints([0, 0, 0, 0, V - 1, V // 2], "cpu"), [0.5, 0.3, 0.6, 0.9999, 1.0, 0.8]
+
+    def halfway(T, k):
+        """The masses as they are, but between those of two tokens: there the target is half a token's mass from either, more than
+        the rounding of all terms by 2^-24 makes (two of the whole, 151,936 tokens: 0.02 of a token's mass where all are alike)."""
+        made = []
+        for r in range(6):
+            x = (logits[r] * (torch.tensor(1.0) / T)).double().sort(descending=True).values[:k[r] or V]
+            upto = torch.cumsum(torch.exp(x - x[0]), 0)
+            at = int((upto >= p[r] * upto[-1]).nonzero()[0])
+            made.append(float((upto[at] + upto[at - 1]) / 2 / upto[-1]) if p[r] < 1 else 1.0)
+        return torch.tensor(made)
+
+    check_probabilities(logits, 20 * T, None, halfway(20.0, [0] * 6))
+    p = halfway(1.0, k.tolist())
+    check_probabilities(logits, T, k, p)
+    args = logits.to(DEV), T.to(DEV), k.to(DEV), p.to(DEV)
+    first, again = torch.empty(6, V, device=DEV), torch.empty(6, V, device=DEV)
+    ops.probabilities(args[0], first, *args[1:])
+    for _ in range(5):
+        ops.probabilities(args[0], again, *args[1:])
+        assert torch.equal(first, again)
+
+
+@gpu
+@pytest.mark.parametrize("V", [5, 1027, 30002])
+def test_probabilities_of_rows_that_begin_anywhere(V):
+    g = torch.Generator().manual_seed(V)
+    rows, T = 3 * torch.randn(4, V, generator=g), torch.tensor([0.7, 0.0, 1.2, 0.9])
+    k, p = ints([0, 3, 20, 0], "cpu"), torch.tensor([0.8, 1.0, 0.9, 1.0])
+    want = plain_probabilities(rows, T, k, p)
+    for a, b in ((1, 0), (0, 3), (2, 2), (3, 1)):
+        logits, out = torch.full((4 * V + 8,), 50.0, device=DEV), torch.full((4 * V + 8,), 7.0, device=DEV)
+        logits[a:a + 4 * V] = rows.view(-1).to(DEV)
+        ops.probabilities(logits[a:a + 4 * V].view(4, V), out[b:b + 4 * V].view(4, V), T.to(DEV), k.to(DEV), p.to(DEV))
+        got = out[b:b + 4 * V].view(4, V).cpu().double()
+        assert ((got > 0) == (want > 0)).all() and ((got - want).abs() <= 2.8e-6 * want).all()
+        assert (out[:b] == 7.0).all() and (out[b + 4 * V:] == 7.0).all()
 
 
 @gpu
@@ -761,6 +842,41 @@ def test_the_step_replays_from_a_graph():
 
 
 @gpu
+def test_calls_on_two_streams_at_once():
+    """Each has its own workspace, and a verification whose blocks wait for each other shares the chip with another's."""
+    made = [make_drafts([9, 1, 6, 0, 30] * 8, 20001, seed, True, near=1.0) for seed in (1, 2)]
+    on = [[x.to(DEV) if torch.is_tensor(x) else ints(x) for x in m] for m in made]
+    steps = [make_step(BF16, 14, 2, 64, 16, [8, 5, 13], [300, 40, 2000], seed=seed) for seed in (1, 2)]
+    R, N = 40, on[0][0].shape[0]
+    T, pr = torch.full((N,), 0.8, device=DEV), torch.full((N,), 0.9, device=DEV)
+
+    def run(i):
+        p, q, tokens, parents, starts, u = on[i]
+        nodes, counts, out = ints([[7] * 30] * R), ints([7] * R), ints([7] * R)
+        made, s = torch.empty_like(p), steps[i]
+        ops.probabilities(p, made, T, None, pr)
+        ops.verify_drafts(p, q, tokens, parents, starts, u, nodes, counts, out)
+        ops.tree_attention(s.q, s.kv, s.ctx, s.tree, s.out, 14, s.scale)
+        return made, nodes, counts, out, s.out.clone()
+
+    want = [run(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(4):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for results in got[i]:
+            for a, b in zip(want[i], results):
+                assert torch.equal(a, b)
+    paths, drawn = plain_verify(*made[0], 30)
+    assert want[0][2].tolist() == [len(x) for x in paths] and want[0][3].tolist() == drawn
+
+
+@gpu
 def test_the_sampler_and_the_pools_reach_them():
     """``Sampler.probabilities`` and ``verify`` against the operators with the same settings; ``CachePools.keep_tokens`` moves the
     entries of every group."""
@@ -892,7 +1008,8 @@ def test_keep_tokens_refuses(host):
                dict(pages=[torch.zeros(2, 7, 3, 16, 8), torch.zeros(2, 7, 3, 8, 16).bfloat16()]), dict(pages=[torch.zeros(7, 3, 16)] * 2),
                dict(pages=[torch.zeros(2, 7, 3, 16, 8).half()] * 2, transposed=[False] * 2), dict(first=torch.zeros(3, dtype=i32)),
                dict(counts=torch.zeros(2, dtype=torch.int64)), dict(nodes=torch.zeros(2, dtype=i32)), dict(table_rows=torch.zeros(3, dtype=i32)),
-               dict(table_rows=None, block_table=torch.zeros(1, 5, dtype=i32)), dict(pages=[torch.zeros(2, 7, 3, 16, 8)] * 17, transposed=[False] * 17)):
+               dict(table_rows=None, block_table=torch.zeros(1, 5, dtype=i32)), dict(pages=[torch.zeros(2, 7, 3, 16, 8)] * 17, transposed=[False] * 17),
+               dict(pages=[torch.zeros(2, 7, 3, 16, 8)] * 2, transposed=[False] * 2)):
         refused(host, lambda: args(**kw))
     args(nodes=torch.zeros(2, 0, dtype=i32))
     assert not host
@@ -930,6 +1047,13 @@ def test_tree_attention_refuses(host):
     refused(host, lambda: args(context_lens=torch.zeros(2)))
     args()
     assert host == ["ms_tree_attention_generic"]
+    wide = dict(q=torch.zeros(6, 128), out=torch.zeros(6, 128), k_pages=torch.zeros(5, 2, 4, 32), v_pages=torch.zeros(5, 2, 4, 32))
+    del host[:]
+    refused(host, lambda: args(max_context_len=9, **wide))
+    refused(host, lambda: args(v_pages=torch.zeros(5, 2, 32, 4), **{k: v for k, v in wide.items() if k != "v_pages"}))
+    refused(host, lambda: args(**{**wide, "out": torch.zeros(6, 128).bfloat16()}))
+    args(**wide)
+    assert host == ["ms_tree_attention_f32"]
 
 
 def test_pools_that_cannot_drop_tokens_refuse(host):
