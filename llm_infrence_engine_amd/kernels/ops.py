@@ -1554,6 +1554,8 @@ def tree_attention_generic(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     N = q.shape[0]
     if n_live_tokens is not None:
         _need(n_live_tokens, "n_live_tokens", torch.int32, (1,), _device())
+    if N == 0 or context_lens.shape[0] == 0:
+        return out
     _call("ms_tree_attention_generic", q.data_ptr(), q_stride, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
           block_table.shape[1], _ptr(table_rows), token_req.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(),
           _ptr(n_live_tokens), tree.data_ptr(), words, out.data_ptr(), num_heads * dv, N, num_heads, nkv, d, dv, page_size,

@@ -816,7 +816,7 @@ def test_the_step_replays_from_a_graph():
         step()
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph, stream=side):
+    with torch.inference_mode(), torch.cuda.graph(graph, stream=side):     # (as the engine captures: the generator keeps the first mode)
         step()
     results = []
     for i in range(1, 4):
@@ -839,6 +839,30 @@ def test_the_step_replays_from_a_graph():
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
         results.append(both[0][3].tolist())
     assert results[0] != results[1] or results[1] != results[2]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_calls_without_requests_or_tokens(dtype):
+    """No requests: tokens that pad the batch stay; requests without tokens: empty paths, no token, nothing moved."""
+    for d in (64, 48):
+        s = make_step(dtype, 4, 2, d, 16, [3], [20])
+        s.ctx.q_start, s.ctx.context_lens, s.kv.table_rows = ints([0]), ints([]), ints([])
+        ops.tree_attention(s.q, s.kv, s.ctx, s.tree, s.out, 4, s.scale)
+        assert (s.out == 7.0).all()
+        s = make_step(dtype, 4, 2, d, 16, [0, 0], [20, 0])
+        assert ops.tree_attention(s.q, s.kv, s.ctx, s.tree, s.out, 4, s.scale).shape == (0, 4 * d)
+    assert ops.probabilities(torch.empty(0, 50, device=DEV), torch.empty(0, 50, device=DEV)).shape == (0, 50)
+    for with_q in (True, False):
+        q = torch.empty(0, 50) if with_q else None
+        nodes, counts, out = run_verify(torch.empty(0, 50), q, [], [], [0, 0, 0], torch.empty(0), 3)
+        assert nodes == [[-1] * 3] * 2 and counts == [0, 0] and out == [-1, -1]
+    none = ints([])
+    ops.verify_drafts(torch.empty(0, 50, device=DEV), None, none, none, ints([0]), torch.empty(0, device=DEV), none.view(0, 3), none, none)
+    pages, table, _ = make_pages(dtype, 2, 2, 64, 16, [40, 20], False)
+    got = pages.to(DEV)
+    ops.keep_tokens([got], [False], table.to(DEV), ints([30, 15]), ints(nodes), ints(counts))
+    assert torch.equal(got.cpu(), pages)
 
 
 @gpu
