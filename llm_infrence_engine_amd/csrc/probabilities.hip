@@ -4,7 +4,8 @@
 //
 // The work is two readings of the logits and one writing; the rest is to find the floor, the smallest value kept, in few
 // launches and without a sort.  A row is spread over n_chunks blocks; with `target` = top_p times the mass that top-k keeps:
-//   1 every chunk's maximum; with a top-k also the maxima of groups of a wave's lanes (as many groups as four times k or so)
+//   1 every chunk's maximum; with a top-k also the maxima of groups of a wave's lanes (as many groups as four times k or so); with
+//     neither top-k nor top-p the chunk's mass against its maximum too, and 4 is next (33 rows of 100,003: 18 us, in three launches 26)
 //   2 top-k: the k-th largest group maximum is no larger than the k-th largest value, and only a few more than k values are above
 //     it (50 of 384 groups: 54 expected): these are collected as candidates, those equal to it counted
 //     top-p alone: every chunk's mass, and a histogram of masses by the distance from the maximum (1/128 wide, 2,048 of them), joined
@@ -195,6 +196,32 @@ probabilities_max_kernel(const float* __restrict__ logits, size_t ld, int V, con
     }
     return;
   }
+  if (!a.k && !a.use_p) {
+    // nothing to look for: the mass with the maximum, every thread's against its own so far, joined against the chunk's
+    __shared__ float red_f[WAVES];
+    __shared__ double red_d[WAVES];
+    float most = -INFINITY;
+    double sum = 0.0;
+    for_quads(row, V, begin, end, [&](int, const float4& v) {
+      const float s[4] = {v.x * a.inv_t, v.y * a.inv_t, v.z * a.inv_t, v.w * a.inv_t};
+      const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));      // (NaN never wins)
+      if (top > most) {
+        sum *= (double)exp_of(most - top);
+        most = top;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += (double)exp_of(s[i] - most);
+    });
+    float best = most;
+    for (int o = MS_WAVE / 2; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor(best, o, MS_WAVE));
+    if (lane == 0) red_f[wave] = best;
+    __syncthreads();
+    best = red_f[0];
+    for (int k = 1; k < WAVES; ++k) best = fmaxf(best, red_f[k]);
+    sum = block_sum_double(sum * (double)exp_of(most - best), red_d);
+    if (threadIdx.x == 0) { w.chunk_max[c] = order_key(best); w.chunk_mass[c] = sum; }
+    return;
+  }
   if (c == 0 && threadIdx.x == 0) { w.n_candidates = 0u; w.n_ties = 0u; w.bin = -1; w.bound = 0u; }
   if (threadIdx.x == 0) { w.chunk_mass[c] = 0.0; w.chunk_above[c] = 0.0; }
   if (a.use_p && !a.k && !a.all)
@@ -251,13 +278,13 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
   const int r = blockIdx.y, c = blockIdx.x;
   RowWork& w = work[r];
   const RowPlan a = plan_of(temperature, top_k, top_p, r, V, n_chunks);
-  if (a.greedy) return;
+  if (a.greedy || (!a.k && !a.use_p)) return;
   const float* row = logits + (size_t)r * ld;
   int begin, end;
   quad_range(row, V, n_chunks, c, &begin, &end);
   const float zmax = key_value(largest_key(w, n_chunks));
   if (!finite(zmax)) return;      // no mass: the last kernel puts a one where the greedy choice stands
-  if ((a.k || a.use_p) && a.all) {
+  if (a.all) {
     here.begin();
     for_values(row, V, begin, end, [&](float v) {
       const float s = v * a.inv_t;
@@ -319,29 +346,25 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
     return;
   }
   double mine = 0.0;
-  if (!a.use_p) {
-    for_values(row, V, begin, end, [&](float v) { mine += (double)exp_of(v * a.inv_t - zmax); });
-  } else {
-    // In LDS a value adds to its bin, as a whole number, what its mass is of the mass at the bin's beginning, e^-f at f behind it (f <
-    // 1/128: 1 - f + f^2/2 is off by 2^-23); as many places as a bin of all of the chunk's values has room for.  Float additions in
-    // LDS took 5 times as long as whole ones (20 M values into 2,048 bins: 107 us, 23, the reading alone 23).
-    const int places = min(20, __builtin_clz(4 * max(1, end - begin)) - 1);
-    const float whole = (float)(1 << places);
-    for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0u;
-    __syncthreads();
-    for_values(row, V, begin, end, [&](float v) {
-      const float s = v * a.inv_t, x = (zmax - s) * BINS_A_UNIT;
-      mine += (double)exp_of(s - zmax);
-      if (x < (float)BINS) {
-        const int bin = (int)x;
-        const float f = (x - (float)bin) * (1.0f / BINS_A_UNIT);
-        atomicAdd(&hist[bin], (unsigned)(fmaf(fmaf(0.5f, f, -1.0f), f, 1.0f) * whole + 0.5f));
-      }
-    });
-    __syncthreads();
-    for (int i = threadIdx.x; i < BINS; i += THREADS)
-      if (hist[i]) unsafeAtomicAdd(&w.hist[i], (float)hist[i] / whole * exp_of((float)i * (-1.0f / BINS_A_UNIT)));
-  }
+  // In LDS a value adds to its bin, as a whole number, what its mass is of the mass at the bin's beginning, e^-f at f behind it (f <
+  // 1/128: 1 - f + f^2/2 is off by 2^-23); as many places as a bin of all of the chunk's values has room for.  Float additions in
+  // LDS took 5 times as long as whole ones (20 M values into 2,048 bins: 107 us, 23, the reading alone 23).
+  const int places = min(20, __builtin_clz(4 * max(1, end - begin)) - 1);
+  const float whole = (float)(1 << places);
+  for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0u;
+  __syncthreads();
+  for_values(row, V, begin, end, [&](float v) {
+    const float s = v * a.inv_t, x = (zmax - s) * BINS_A_UNIT;
+    mine += (double)exp_of(s - zmax);
+    if (x < (float)BINS) {
+      const int bin = (int)x;
+      const float f = (x - (float)bin) * (1.0f / BINS_A_UNIT);
+      atomicAdd(&hist[bin], (unsigned)(fmaf(fmaf(0.5f, f, -1.0f), f, 1.0f) * whole + 0.5f));
+    }
+  });
+  __syncthreads();
+  for (int i = threadIdx.x; i < BINS; i += THREADS)
+    if (hist[i]) unsafeAtomicAdd(&w.hist[i], (float)hist[i] / whole * exp_of((float)i * (-1.0f / BINS_A_UNIT)));
   mine = block_sum_double(mine, red_d);
   if (threadIdx.x == 0) w.chunk_mass[c] = mine;
 }
@@ -522,7 +545,10 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
 
   Kept kept = {0u, 0.0};
   if (!a.k && !a.use_p) {
-    kept.mass = sum_of(w.chunk_mass, n_chunks);
+    const int lane = threadIdx.x & (MS_WAVE - 1);
+    double v = lane < n_chunks ? w.chunk_mass[lane] * (double)exp_of(key_value(w.chunk_max[lane]) - zmax) : 0.0;
+    for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
+    kept.mass = __shfl(v, 0, MS_WAVE);
   } else {
     // A candidate knows how many are larger, and their mass.  Top-k keeps it if these are fewer than k; top-p if what is larger has
     // not reached the target.  Values equal to the bound are one candidate more, as often as they were counted.
@@ -637,7 +663,7 @@ extern "C" int ms_probabilities(const float* logits, long long ld, int n_rows, i
   n_chunks = std::max(1, std::min(std::min(n_chunks, MAX_CHUNKS), (vocab + 2047) / 2048));
   const dim3 grid(n_chunks, n_rows), block(THREADS);
   probabilities_max_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks);
-  probabilities_collect_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks);
+  if (top_k || top_p) probabilities_collect_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks);
   if (top_p) probabilities_near_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks);
   probabilities_write_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks, out, (size_t)out_ld);
   return ms_launch_status();
