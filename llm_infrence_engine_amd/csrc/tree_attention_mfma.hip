@@ -11,10 +11,11 @@
 // where row r of the u-th score product of a unit of 32 keys is its key 8 (r / 4) + 4 u + r % 4, so that a lane (quarter kq)
 // holds the scores of the keys 8 kq .. + 7 and needs one 16-byte read of a value's row.  Keys from before the step are visible
 // to every column; only units that reach into the step's own entries (the last ones) look at the mask.
-// Rounding: the weights e^(s - ref) meet the values as bfloat16, since that is what the product takes; each is off by 2^-8 of
-// itself at most, and the sum that divides is of the rounded ones.  Scores, exponentials, sums and results up to the last
-// rounding are float.  Against 64 bits the result is off by 0.0019 of its norm (a tree of 8 behind 192 keys) to
-// 0.0023 (4 of up to 63 behind 16,011); the same in float with the result alone rounded is off by 0.0017.
+// Rounding: the product takes bfloat16, so a weight e^(s - ref) meets the values in two parts, its upper half and what that leaves
+// out, together off by 2^-15 of it at most; the sum that divides is of the same parts.  Scores, exponentials, sums and results up to
+// the last rounding are float: against 64 bits the result is off by 0.0017 of its norm, as one that is rounded at the end alone (with
+// weights of one bfloat16 0.0019 to 0.0023).  The second product of the values costs what it takes: 4 trees of up to 63 behind
+// 16,011 keys 101 -> 127 us, 8 of up to 16 behind 2,000 18.6 -> 19.1, smaller ones nothing.
 // The keys of a request are shared out over n_splits blocks, which leave unnormalised float results that a second kernel
 // adds up: with few columns there is one (request, head) tile for a handful of CUs, and a step waits for the longest chain.
 #include "attention_tiles.h"
@@ -28,6 +29,7 @@ typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void global_void;
 
@@ -44,6 +46,13 @@ __device__ __forceinline__ float column_max(float x) {
   const unsigned w = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
   const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// What the upper half of a weight's bits, a bfloat16 too small by less than 2^-7, leaves out.  2^-21 of the weight comes on top, which
+// all weights have alike, so that it falls out of the result: no rest of a weight above zero is zero, and an infinite value
+// stays infinite.
+__device__ __forceinline__ float rest_of(float weight) {
+  return fmaf(weight, 1.0f + 1.0f / 2097152.0f, -__uint_as_float(__float_as_uint(weight) & 0xffff0000u));
 }
 
 template <int D, int WC, int KG, int NT>
@@ -185,7 +194,7 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
     return left >= 8 ? bits : left <= 0 ? 0u : bits & ((1u << left) - 1u);
   };
 
-  // The sums of the exponentials are those of the rounded ones that meet the values: one more product, of P^T with ones.
+  // The sums of the exponentials are those of the parts that meet the values: a product of P^T with ones more for each.
   float m[NT];
   f32x4 o[CT][NT] = {}, lsum[NT] = {};
 #pragma unroll
@@ -297,26 +306,46 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
         for (int c = 0; c < CT; ++c) o[c][t2] *= corr;
       }
     }
-    bf16x8 p[UNITS][NT];
+    // Values are read two fragments ahead of their products, the first ones before the exponentials (4 of up to 63 behind 16,011
+    // keys 131 -> 127 us; the same for the keys made no difference).
+    const auto values = [&](int f) { return *reinterpret_cast<const bf16x8*>(st + f / CT * 2 * CHUNK + v_row + f % CT * 256); };
+    bf16x8 now[2] = {values(0), values(1)}, next[2];
+    __builtin_amdgcn_sched_barrier(0);
+    bf16x8 p[UNITS][NT], rest[UNITS][NT];
 #pragma unroll
     for (int n = 0; n < UNITS; ++n)
 #pragma unroll
       for (int t2 = 0; t2 < NT; ++t2) {
         const float ref = m[t2] == -INFINITY ? 0.f : m[t2];
+        u32x4 high;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) p[n][t2][u * 4 + i] = (__bf16)fast_exp2(fmaf(s[n][u][t2][i], scale_log2e, -ref));
+        for (int i = 0; i < 8; i += 2) {
+          const float a = fast_exp2(fmaf(s[n][i / 4][t2][i % 4], scale_log2e, -ref));
+          const float b = fast_exp2(fmaf(s[n][i / 4][t2][i % 4 + 1], scale_log2e, -ref));
+          high[i / 2] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+          rest[n][t2][i] = (__bf16)rest_of(a);
+          rest[n][t2][i + 1] = (__bf16)rest_of(b);
+        }
+        p[n][t2] = __builtin_bit_cast(bf16x8, high);
         lsum[t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[n][t2], lsum[t2], 0, 0, 0);
+        lsum[t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, rest[n][t2], lsum[t2], 0, 0, 0);
       }
 #pragma unroll
-    for (int n = 0; n < UNITS; ++n)
+    for (int f = 0; f < UNITS * CT; f += 2) {
+      if (f + 2 < UNITS * CT) { next[0] = values(f + 2); next[1] = values(f + 3); }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const bf16x8 v = *reinterpret_cast<const bf16x8*>(st + n * 2 * CHUNK + v_row + c * 256);
+      for (int part = 0; part < 2; ++part)
 #pragma unroll
-        for (int t2 = 0; t2 < NT; ++t2) o[c][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[n][t2], o[c][t2], 0, 0, 0);
-      }
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t2 = 0; t2 < NT; ++t2) {
+            const int n = (f + i) / CT, c = (f + i) % CT;
+            o[c][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(now[i], part ? rest[n][t2] : p[n][t2], o[c][t2], 0, 0, 0);
+          }
+      __builtin_amdgcn_sched_barrier(0);
+      now[0] = next[0]; now[1] = next[1];
+    }
     if (masked && spoiled[kg][stage] == t + 1) {       // (rare: the values are read again from where they are)
       int rows = page_size;
       asm volatile("" : "+s"(rows));                   // (nothing of this is worked out ahead of the loop and kept in registers)
@@ -331,7 +360,7 @@ tree_attention_mfma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf
           for (int t2 = 0; t2 < NT; ++t2) {
             float mine = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mine = (k & 7) == i ? (float)p[n][t2][i] : mine;
+            for (int i = 0; i < 8; ++i) mine = (k & 7) == i ? (float)p[n][t2][i] + (float)rest[n][t2][i] : mine;
             const float w = __shfl(mine, owner, MS_WAVE);
             const bool see = (__shfl(sees[n][t2], owner, MS_WAVE) >> (k & 7)) & 1u;
 #pragma unroll
@@ -756,12 +785,12 @@ constexpr Kind KINDS[2][4] = {{{1, 8, 1, 0.75, 0.0}, {2, 4, 1, 0.37, 1.02}, {4, 
 // take.  Narrow kinds share a small step out over the chip, and every block's chain is short; wide ones read the keys less
 // often.  The choice is the least of a model: a launch (4.3 us), then the chains, as often as all blocks take the chip's room, or
 // the keys at 13.5 TB/s (what all tiles of columns drew together, from L2s and memory), whichever is longer, and the second kernel
-// (3.1 us, the parts written and read at 4.4 TB/s).  Its numbers are fitted to the times of all kinds and shares at 44 steps of 64
-// and 128 dims (1 to 64 requests of 1 to 63 tokens behind 64 to 16,011 keys); there its choice takes 1.7% longer than the fastest on
-// average, 15% at most.  us measured, the choice against the fastest and the slowest kind with its best share: 8 tokens of 14
-// heads of 64 on 2 behind 192 keys 6.7, 6.7 (128 columns a block: 9.2); 28 heads of 128 on 4: 8 x 16 behind 2,000 19.0, 19.0
-// (16 columns: 25.1), 32 x 8 behind 1,000 22.5, 20.5 (16 columns: 31.3); 40 on 8: 2 x 16 behind 4,000 19.2, 18.9 (128 columns: 21.1),
-// 4 x 63 behind 16,011 101, 101 (16 columns: 274).
+// (3.1 us, the parts written and read at 4.4 TB/s).  Its numbers were fitted, with weights of one part, to the times of all kinds and
+// shares at 44 steps of 64 and 128 dims (1 to 64 requests of 1 to 63 tokens behind 64 to 16,011 keys), and 32 dims take those of 64;
+// at these steps its choice takes 1.9% longer than the fastest on average, 16% at most.  us measured, the choice against the
+// fastest and the slowest kind with its best share: 8 tokens of 14 heads of 64 on 2 behind 192 keys 7.1, 6.9 (128 columns a
+// block: 9.5); 28 heads of 128 on 4: 8 x 16 behind 2,000 19.8, 19.8 (16 columns: 26.6), 32 x 8 behind 1,000 23.0, 21.1 (16 columns:
+// 32.4); 40 on 8: 2 x 16 behind 4,000 19.6, 19.5 (128 columns: 22.5), 4 x 63 behind 16,011 126, 126 (16 columns: 293).
 extern "C" int ms_tree_attention_mfma_plan(int n_requests, int n_tokens, int max_q_len, int max_context_len, int num_heads,
                                            int num_kv_heads, int head_dim, int page_size) {
   if ((head_dim != 32 && head_dim != 64 && head_dim != 128) || page_size <= 0 || page_size % 16) return -1;

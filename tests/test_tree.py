@@ -279,6 +279,23 @@ def test_tree_attention_of_tokens_that_are_nobodys(dtype, d):
     assert (out[N:] == 3.0).all()
 
 
+@gpu
+@pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (8, 2, 128), (4, 2, 32)])
+@pytest.mark.parametrize("share", [64, 192, 4096])
+def test_tree_attention_weights_are_not_rounded_to_bfloat16(monkeypatch, nh, nkv, d, share):
+    """The result is off by its own rounding, 2^-8 of itself, and hardly more: the weights come in two parts that are off by 2^-15 of
+    a weight together, in the sum of weighted values as in the one that divides (2^-14 of both, second-order terms with it), and
+    scores, exponentials and sums are floats, as the limits of ``close_enough`` have them."""
+    get = ops._get
+    for kind in range(4):
+        monkeypatch.setattr(ops, "_get", lambda name: (lambda *a: kind * 65536 + share // 64) if name == "ms_tree_attention_mfma_plan" else get(name))
+        s = make_step(BF16, nh, nkv, d, 16, [12, 0, 37, 1], [1301, 0, 75, 640], seed=7)
+        ops.tree_attention(s.q, s.kv, s.ctx, s.tree, s.out, s.nh, s.scale)
+        want, size = plain_attention(s)
+        off = (s.out.cpu().double().view(want.shape) - want).abs()
+        assert (off <= 6e-5 + 2.0 ** -8 * want.abs() + 2.0 ** -14 * (size + want.abs())).all(), (kind, off.max())
+
+
 # ------------------------------------------------------------------------------------------------ probabilities
 def plain_probabilities(logits, T, top_k, top_p):
     """float64, row by row; the scaled logits are floats, as the sampler has them."""
