@@ -1580,8 +1580,7 @@ def tree_attention_mfma(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     N, R = q.shape[0], context_lens.shape[0]
     if N == 0 or R == 0:
         return out
-    if max_context_len < 1 or max_context_len > block_table.shape[1] * page_size:
-        raise ValueError(f"max_context_len {max_context_len} does not fit a table of {block_table.shape[1]} pages of {page_size}")
+    _tree_bounds(max_q_len, max_context_len, block_table, page_size)
     if small:
         plan = _get("ms_tree_attention_mfma_plan")(R, N, max_q_len, max_context_len, num_heads, nkv, d, page_size)
         kind, share = plan >> 16, (plan & 0xFFFF) * 64
@@ -1602,6 +1601,12 @@ def tree_attention_mfma(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     else:
         _call("ms_tree_attention_f32", *args, P, float(scale), share, n_splits, _stream())
     return out
+
+
+def _tree_bounds(max_q_len: int, max_context_len: int, block_table: torch.Tensor, page_size: int) -> None:
+    if max_q_len < 1 or max_context_len < max_q_len or max_context_len > block_table.shape[-1] * page_size:
+        raise ValueError(f"max_q_len {max_q_len} / max_context_len {max_context_len} do not fit a table of {block_table.shape[-1]} pages of "
+                         f"{page_size}")
 
 
 def _tree_step(q, k_pages, v_pages, v_shape, block_table, token_req, q_start, context_lens, tree, table_rows, out, num_heads, dv, max_q_len):
@@ -1653,9 +1658,15 @@ def tree_attention(q: torch.Tensor, kv, ctx, tree: torch.Tensor, out: torch.Tens
     those in its row of ``tree``, int32 [N, words]: bit j % 32 of word j / 32 stands for the request's j-th token of the
     step (its ancestors and itself, as a rule; bits behind the tree are ignored).  A token that sees nothing gets zeros.
     The step's keys and values lie in the cache in the order of the tokens (``slot_mapping``), encoded with whatever
-    positions the tree gives them; ``keep_tokens`` moves together what is accepted."""
+    positions the tree gives them; ``keep_tokens`` moves together what is accepted.  The context's ``max_q_len`` and
+    ``max_context_len`` bound the trees and the entries; a step with tokens has both."""
     d, page_size = kv.k_pages.shape[3], kv.k_pages.shape[2]
     dv = kv.v_pages.shape[2] if kv.v_transposed else kv.v_pages.shape[3]
+    max_q_len, max_context_len = ctx.max_q_len, ctx.max_context_len
+    if q.shape[0] == 0 or ctx.context_lens.shape[0] == 0:
+        max_q_len, max_context_len = max(1, max_q_len), max(1, max_context_len)
+    else:
+        _tree_bounds(max_q_len, max_context_len, kv.block_table, page_size)
     if q.dtype == torch.bfloat16:
         takes, per = kv.v_transposed and page_size % 16 == 0, 8
     else:
@@ -1663,9 +1674,9 @@ def tree_attention(q: torch.Tensor, kv, ctx, tree: torch.Tensor, out: torch.Tens
     if takes and d == dv and d in (32, 64, 128) and scale > 0 and (q.shape[0] == 1 or q.stride(0) % per == 0) and \
             (kv.k_pages.data_ptr() | kv.v_pages.data_ptr() | q.data_ptr() | out.data_ptr()) % 16 == 0:
         return tree_attention_mfma(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.q_start, ctx.context_lens, tree, out,
-                                   num_heads, scale, max(1, ctx.max_q_len), max(1, ctx.max_context_len), kv.table_rows)
+                                   num_heads, scale, max_q_len, max_context_len, kv.table_rows)
     return tree_attention_generic(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.q_start, ctx.context_lens, tree,
-                                  out, num_heads, scale, max(1, ctx.max_q_len), kv.v_transposed, kv.table_rows, ctx.n_live_tokens)
+                                  out, num_heads, scale, max_q_len, kv.v_transposed, kv.table_rows, ctx.n_live_tokens)
 
 
 def verify_drafts(p: torch.Tensor, q: Optional[torch.Tensor], token_ids: torch.Tensor, parents: torch.Tensor,

@@ -1097,6 +1097,33 @@ def test_tree_attention_refuses(host):
     assert host == ["ms_tree_attention_f32"]
 
 
+def tree_call(width=24, N=6, R=2, **kw):
+    """``tree_attention`` of host tensors: width 24 goes to the kernel for any size, 32 to the matrix cores; ``kw`` goes to the view where it
+    has such a field, else to the context."""
+    from llm_infrence_engine_amd.parts.base import KVView, StepContext
+
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32)     # noqa: E731
+    pages = torch.zeros(5, 2, 4, width), torch.zeros(5, 2, 4, width)
+    kv = KVView({"k": pages[0], "v": pages[1]}, {"k": False, "v": False}, z(3, 2), z(N), table_rows=z(R))
+    ctx = StepContext(N, R, z(N), z(N), z(N), z(R + 1), z(R), z(R), z(N), 4, 8)
+    for name, value in kw.items():
+        setattr(kv if hasattr(kv, name) else ctx, name, value)
+    return ops.tree_attention(torch.zeros(N, 4 * width), kv, ctx, z(N, 1), torch.zeros(N, 4 * width), 4, 0.5)
+
+
+@pytest.mark.parametrize("width,kernel", [(24, "ms_tree_attention_generic"), (32, "ms_tree_attention_f32")])
+def test_tree_attention_refuses_steps_without_bounds(host, width, kernel):
+    """A step with tokens says how long its trees and contexts are at most (its context has 0 for both unless told)."""
+    for kw in (dict(max_q_len=0), dict(max_context_len=0), dict(max_q_len=0, max_context_len=0), dict(max_context_len=3), dict(max_context_len=9)):
+        refused(host, lambda: tree_call(width, **kw))
+    assert tree_call(width, N=0, max_q_len=0, max_context_len=0).shape == (0, 4 * width)
+    tree_call(width, R=0, max_q_len=0, max_context_len=0)
+    assert not host
+    tree_call(width)
+    tree_call(width, max_context_len=4)
+    assert host == [kernel] * 2
+
+
 def test_pools_that_cannot_drop_tokens_refuse(host):
     from llm_infrence_engine_amd.cache.pools import CachePools
 
