@@ -1659,7 +1659,12 @@ def tree_attention(q: torch.Tensor, kv, ctx, tree: torch.Tensor, out: torch.Tens
     step (its ancestors and itself, as a rule; bits behind the tree are ignored).  A token that sees nothing gets zeros.
     The step's keys and values lie in the cache in the order of the tokens (``slot_mapping``), encoded with whatever
     positions the tree gives them; ``keep_tokens`` moves together what is accepted.  The context's ``max_q_len`` and
-    ``max_context_len`` bound the trees and the entries; a step with tokens has both."""
+    ``max_context_len`` bound the trees and the entries; a step with tokens has both.
+
+    There is no window, sink, softcap, slope or gate here as ``paged_attention`` has them.  A view with a window is refused (the
+    pages that it has passed are given back and stand for nothing), and so is one whose entries stand for several tokens."""
+    if getattr(kv, "window", None) or getattr(kv, "stride", 1) != 1:
+        raise ValueError(f"attention over trees has no window ({kv.window}) and takes entries of one token ({kv.stride})")
     d, page_size = kv.k_pages.shape[3], kv.k_pages.shape[2]
     dv = kv.v_pages.shape[2] if kv.v_transposed else kv.v_pages.shape[3]
     max_q_len, max_context_len = ctx.max_q_len, ctx.max_context_len

@@ -1124,6 +1124,14 @@ def test_tree_attention_refuses_steps_without_bounds(host, width, kernel):
     assert host == [kernel] * 2
 
 
+@pytest.mark.parametrize("width", [24, 32])
+def test_tree_attention_refuses_views_with_a_window_or_entries_of_several_tokens(host, width):
+    for kw in (dict(window=4), dict(window=4096), dict(stride=2)):
+        refused(host, lambda: tree_call(width, **kw))
+    tree_call(width, window=None, stride=1)
+    assert len(host) == 1
+
+
 def test_pools_that_cannot_drop_tokens_refuse(host):
     from llm_infrence_engine_amd.cache.pools import CachePools
 
