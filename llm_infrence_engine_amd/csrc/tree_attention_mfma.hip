@@ -490,7 +490,7 @@ tree_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ 
       const int at = s0 + s;
       const float w = at < used ? __shfl(at < MS_WAVE ? m[0] : m[1], at & (MS_WAVE - 1), MS_WAVE) : 0.f;
 #pragma unroll
-      for (int e = 0; e < DL; ++e) acc[e] = fmaf(w, part[s][e], acc[e]);
+      for (int e = 0; e < DL; ++e) acc[e] = fmaf(w, at < used ? part[s][e] : 0.f, acc[e]);      // (behind the last: it again, which may be infinite)
     }
   }
   const float inv = den != 0.f ? 1.0f / den : 0.f;

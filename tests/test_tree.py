@@ -296,6 +296,33 @@ def test_tree_attention_weights_are_not_rounded_to_bfloat16(monkeypatch, nh, nkv
         assert (off <= 6e-5 + 2.0 ** -8 * want.abs() + 2.0 ** -14 * (size + want.abs())).all(), (kind, off.max())
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+@pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (8, 2, 128), (4, 2, 32), (6, 1, 20)])
+def test_tree_attention_of_infinite_values(monkeypatch, dtype, bad, nh, nkv, d):
+    """A visible value that is infinite makes the result infinite, not NaN, however the keys are shared out (every weight is far from
+    underflow: a score is 1.5 times a normal number); one cached before the step does so for all."""
+    get = ops._get
+    trees, contexts = [9, 24], [640, 1170]
+    sees = [ancestors(random_tree(random.Random(4), n)) for n in trees]
+    for share in (128, 256, 384, 2048):
+        forced = {"ms_tree_attention_mfma_plan": 2 * 65536 + share // 64, "ms_tree_attention_f32_share": share}
+        monkeypatch.setattr(ops, "_get", lambda name: (lambda *a: forced[name]) if name in forced else get(name))
+        for at, seen in ((contexts[1] - trees[1] + 13, [i for i in range(24) if 13 in sees[1][i]]), (70, range(24))):
+            s = make_step(dtype, nh, nkv, d, 16, trees, contexts, seed=6, sees=sees)
+            page, slot = int(s.kv.block_table[s.kv.table_rows[1], at // 16]), at % 16
+            if s.kv.v_transposed:
+                s.kv.v_pages[page, :, :, slot] = bad
+            else:
+                s.kv.v_pages[page, :, slot] = bad
+            ops.tree_attention(s.q, s.kv, s.ctx, s.tree, s.out, s.nh, s.scale)
+            got = s.out.cpu().float()
+            for n in range(s.starts[-1]):
+                hit = n >= 9 and n - 9 in seen
+                assert (got[n] == bad).all() if hit else torch.isfinite(got[n]).all(), (share, at, n)
+
+
 # ------------------------------------------------------------------------------------------------ probabilities
 def plain_probabilities(logits, T, top_k, top_p):
     """float64, row by row; the scaled logits are floats, as the sampler has them."""
