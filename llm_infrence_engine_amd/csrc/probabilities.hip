@@ -1,6 +1,7 @@
 // The distributions that tokens are drawn from, whole: out[r, i] = e^(s_i - max) / sum over the kept e^(s_j - max) for the kept
-// i of row r and 0 for the others, s = logits / temperature.  What is kept is decided as in csrc/sampling.hip, with masses e^(s -
-// max) in fixed point whose sums are exact; a row without temperature is a one at its first maximum.
+// i of row r and 0 for the others, s = logits / temperature.  What is kept is what csrc/sampling.hip keeps, token by token: the masses
+// e^(s - max) that decide are its own (fixed_mass) and their sums exact, whoever adds them up in which order; a row without
+// temperature is a one at its first maximum.
 //
 // The work is two readings of the logits and one writing; the rest is to find the floor, the smallest value kept, in few
 // launches and without a sort.  A row is spread over n_chunks blocks; with `target` = top_p times the mass that top-k keeps:
@@ -11,7 +12,7 @@
 //     top-p alone: every chunk's mass, and a histogram of masses by the distance from the maximum (1/128 wide, 2,048 of them), joined
 //     in float: its sums depend on the order, so it only says where to look
 //   3 top-p alone: the values of the histogram's bin in which the target falls, with a neighbour's where it falls that near its
-//     edge, are the candidates; the mass above them is summed up anew, in double
+//     edge, are the candidates; the mass above them is summed up anew
 //   4 a thread to a candidate: count and mass of the larger ones say whether it is kept, the least kept one is the floor (from many
 //     candidates a radix descent over their keys finds it); then every block writes its chunk
 // What the candidates cannot decide (more than MAX_CANDIDATES of them, a k beyond half the groups, a target outside the
@@ -22,10 +23,6 @@
 #include "api.h"
 #include <algorithm>
 #include <type_traits>
-
-// A scaled logit is rounded to a float before anything else is done with it: its key, its mass and its probability are those of one
-// number, wherever they are worked out (a product joined with the subtraction of the maximum is another one).
-#pragma clang fp contract(off)
 
 namespace {
 
@@ -40,8 +37,9 @@ struct RowWork {                       // one per row, in the workspace the call
   unsigned n_candidates, n_ties;       // ties: values equal to the bound
   unsigned bound;                      // top-k: every value above it is a candidate
   int bin;                             // top-p alone: the middle bin of the candidates, < 0: none
-  double chunk_mass[MAX_CHUNKS];
-  double chunk_above[MAX_CHUNKS];      // mass of the values above the candidates'
+  double chunk_sum[MAX_CHUNKS];        // neither top-k nor top-p: of the exponentials, against the chunk's own maximum
+  unsigned long long chunk_mass[MAX_CHUNKS];
+  unsigned long long chunk_above[MAX_CHUNKS];      // mass of the values above the candidates'
   int chunk_first[MAX_CHUNKS];         // no temperature: where the largest stands
   unsigned candidates[MAX_CANDIDATES];          // keys
   float hist[BINS];
@@ -124,11 +122,11 @@ __device__ __forceinline__ float exp_of(float x) {
   return fmaf(e * 0.693147181f, r, e);
 }
 
-// The mass of a candidate, cut to 44 binary places: candidates come in no particular order, and sums of these do not depend on it.
-// (Sums over a row, which are made in one order, are sums of the exponentials as doubles: a third of the work.)
-__device__ __forceinline__ unsigned long long mass_of(float s, float zmax) {
-  return (unsigned long long)(exp_of(s - zmax) * (float)(1ull << FIX_PLACES));
+// fixed_mass as a double (NaN: none): a thread adds up to 512 of them without rounding, 2^53, in a third of the instructions.
+__device__ __forceinline__ double whole_mass(float s, float zmax) {
+  return (double)truncf(expf(fmaxf(s - zmax, -200.f)) * (float)(1ull << FIX_PLACES));
 }
+constexpr int EXACT_SUMS = 512 * THREADS;      // values a chunk
 constexpr double MASS_UNIT = 1.0 / (double)(1ull << FIX_PLACES);
 
 __device__ double block_sum_double(double v, double* red) {
@@ -158,9 +156,9 @@ __device__ __forceinline__ unsigned largest_key(const RowWork& w, int n_chunks) 
   for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) best = max(best, (unsigned)__shfl_xor((int)best, o, MS_WAVE));
   return __builtin_amdgcn_readfirstlane(best);
 }
-__device__ __forceinline__ double sum_of(const double* chunks, int n_chunks) {
+__device__ __forceinline__ unsigned long long sum_of(const unsigned long long* chunks, int n_chunks) {
   const int lane = threadIdx.x & (MS_WAVE - 1);
-  double v = lane < n_chunks ? chunks[lane] : 0.0;
+  unsigned long long v = lane < n_chunks ? chunks[lane] : 0ull;
   for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
   return __shfl(v, 0, MS_WAVE);
 }
@@ -219,11 +217,11 @@ probabilities_max_kernel(const float* __restrict__ logits, size_t ld, int V, con
     best = red_f[0];
     for (int k = 1; k < WAVES; ++k) best = fmaxf(best, red_f[k]);
     sum = block_sum_double(sum * (double)exp_of(most - best), red_d);
-    if (threadIdx.x == 0) { w.chunk_max[c] = order_key(best); w.chunk_mass[c] = sum; }
+    if (threadIdx.x == 0) { w.chunk_max[c] = order_key(best); w.chunk_sum[c] = sum; }
     return;
   }
   if (c == 0 && threadIdx.x == 0) { w.n_candidates = 0u; w.n_ties = 0u; w.bin = -1; w.bound = 0u; }
-  if (threadIdx.x == 0) { w.chunk_mass[c] = 0.0; w.chunk_above[c] = 0.0; }
+  if (threadIdx.x == 0) { w.chunk_mass[c] = 0ull; w.chunk_above[c] = 0ull; }
   if (a.use_p && !a.k && !a.all)
     for (int i = c * THREADS + threadIdx.x; i < BINS; i += n_chunks * THREADS) w.hist[i] = 0.f;
   unsigned best = 0;
@@ -272,7 +270,6 @@ __global__ void __launch_bounds__(THREADS)
 probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
                              const int* __restrict__ top_k, const float* __restrict__ top_p, RowWork* __restrict__ work, int n_chunks) {
   __shared__ unsigned long long red[WAVES];
-  __shared__ double red_d[WAVES];
   __shared__ unsigned hist[BINS];
   __shared__ Candidates here;
   const int r = blockIdx.y, c = blockIdx.x;
@@ -355,7 +352,7 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
   __syncthreads();
   for_values(row, V, begin, end, [&](float v) {
     const float s = v * a.inv_t, x = (zmax - s) * BINS_A_UNIT;
-    mine += (double)exp_of(s - zmax);
+    mine += whole_mass(s, zmax);
     if (x < (float)BINS) {
       const int bin = (int)x;
       const float f = (x - (float)bin) * (1.0f / BINS_A_UNIT);
@@ -365,8 +362,8 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += THREADS)
     if (hist[i]) unsafeAtomicAdd(&w.hist[i], (float)hist[i] / whole * exp_of((float)i * (-1.0f / BINS_A_UNIT)));
-  mine = block_sum_double(mine, red_d);
-  if (threadIdx.x == 0) w.chunk_mass[c] = mine;
+  const unsigned long long mass = block_sum_u64((unsigned long long)mine, red);
+  if (threadIdx.x == 0) w.chunk_mass[c] = mass;
 }
 
 // What the mass of the larger values must not have reached: top_p times the whole, and a unit of mass at least, so that the largest
@@ -375,13 +372,12 @@ __device__ __forceinline__ unsigned long long target_of(float p, unsigned long l
   const double target = (double)p * (double)total;
   return target >= 1.0 ? (unsigned long long)target : 1ull;
 }
-__device__ __forceinline__ double target_of(float p, double total) { return fmax((double)p * total, MASS_UNIT); }
 
 // ---- 3
 __global__ void __launch_bounds__(THREADS)
 probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, const float* __restrict__ temperature,
                           const int* __restrict__ top_k, const float* __restrict__ top_p, RowWork* __restrict__ work, int n_chunks) {
-  __shared__ double red[WAVES];
+  __shared__ unsigned long long red[WAVES];
   __shared__ float wave_sum_sm[WAVES];
   __shared__ int found, up, down;      // the target's bin; those before and behind it that count too
   __shared__ Candidates here;
@@ -391,7 +387,7 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   if (a.greedy || a.k || !a.use_p || a.all) return;
   const float zmax = key_value(largest_key(w, n_chunks));
   if (!finite(zmax)) return;
-  const double whole = sum_of(w.chunk_mass, n_chunks);
+  const double whole = (double)sum_of(w.chunk_mass, n_chunks) * MASS_UNIT;
   const float target = (float)((double)a.p * whole), near = (float)whole * NEAR_EDGE;
   // the first bin at which the running mass reaches the target; a thread owns two bins
   const float h0 = w.hist[2 * threadIdx.x], h1 = w.hist[2 * threadIdx.x + 1];
@@ -423,15 +419,15 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   here.begin();
   for_values(row, V, begin, end, [&](float v) {
     const float s = v * a.inv_t;
-    if (s > high) above += (double)exp_of(s - zmax);
+    if (s > high) above += whole_mass(s, zmax);
     else if (s >= low) here.add(order_key(s));
   });
   here.hand_over(w);
-  above = block_sum_double(above, red);
-  if (threadIdx.x == 0) w.chunk_above[c] = above;
+  const unsigned long long mass = block_sum_u64((unsigned long long)above, red);
+  if (threadIdx.x == 0) w.chunk_above[c] = mass;
 }
 
-struct Kept { unsigned floor; double mass; };
+struct Kept { unsigned floor; unsigned long long mass; };
 
 // The floor among what `each` hands to its function, scaled logits in any order (NaN: nobody), and the mass of what is kept: a radix
 // descent of the block over their keys.  `need`, from the mass that top-k keeps, is what the larger values' must not have reached.
@@ -453,7 +449,7 @@ __device__ __forceinline__ Kept descend(const Each& each, int k, bool use_p, con
         const unsigned key = order_key(s);
         const bool in = s == s && key >= least && (level == 1 || (key >> (shift + (level == 2 ? 11 : 10))) == digits);
         const int bin = (int)((key >> shift) & (unsigned)(bins - 1));
-        unsigned long long m = in ? mass_of(s, zmax) : 0ull;
+        unsigned long long m = in ? fixed_mass(s, zmax) : 0ull;
         const unsigned long long who = __ballot(in);
         if (!who) return;
         const int leader = __builtin_ctzll(who);
@@ -480,15 +476,15 @@ __device__ __forceinline__ Kept descend(const Each& each, int k, bool use_p, con
     floor = search(false, (unsigned long long)k, 0u);
   } else {
     unsigned long long mine = 0ull;
-    each([&](float s) { mine += s == s ? mass_of(s, zmax) : 0ull; });
+    each([&](float s) { mine += s == s ? fixed_mass(s, zmax) : 0ull; });
     total = block_sum_u64(mine, red);
   }
   if (use_p) {
     const unsigned long long need = need_of(total);
-    if (need == 0ull || need > total) return Kept{0u, 0.0};      // (it does not fall among them)
+    if (need == 0ull || need > total) return Kept{0u, 0ull};      // (it does not fall among them)
     floor = search(true, need, floor);
   }
-  return Kept{floor, (double)total * MASS_UNIT};
+  return Kept{floor, total};
 }
 
 // ---- 4
@@ -543,12 +539,13 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
     return;
   }
 
-  Kept kept = {0u, 0.0};
+  Kept kept = {0u, 0ull};
+  double kept_sum;
   if (!a.k && !a.use_p) {
     const int lane = threadIdx.x & (MS_WAVE - 1);
-    double v = lane < n_chunks ? w.chunk_mass[lane] * (double)exp_of(key_value(w.chunk_max[lane]) - zmax) : 0.0;
+    double v = lane < n_chunks ? w.chunk_sum[lane] * (double)exp_of(key_value(w.chunk_max[lane]) - zmax) : 0.0;
     for (int o = MAX_CHUNKS / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MS_WAVE);
-    kept.mass = __shfl(v, 0, MS_WAVE);
+    kept_sum = __shfl(v, 0, MS_WAVE);
   } else {
     // A candidate knows how many are larger, and their mass.  Top-k keeps it if these are fewer than k; top-p if what is larger has
     // not reached the target.  Values equal to the bound are one candidate more, as often as they were counted.
@@ -556,9 +553,9 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
     bool known = n <= MAX_CANDIDATES && (a.all || (a.k ? a.groups > 0 : w.bin >= 0));
     const bool tied = a.k && !a.all, above_them = !a.k && !a.all;
     const unsigned ties = tied ? w.n_ties : 0u, bound = w.bound;
-    const unsigned long long tie_mass = tied ? ties * mass_of(key_value(bound), zmax) : 0ull;
+    const unsigned long long tie_mass = tied ? ties * fixed_mass(key_value(bound), zmax) : 0ull;
     const bool ties_in_k = ties > 0 && n < a.k;
-    const double above = above_them ? sum_of(w.chunk_above, n_chunks) : 0.0, whole = above_them ? sum_of(w.chunk_mass, n_chunks) : 0.0;
+    const unsigned long long above = above_them ? sum_of(w.chunk_above, n_chunks) : 0ull, whole = above_them ? sum_of(w.chunk_mass, n_chunks) : 0ull;
     unsigned mine = 0u;
     unsigned long long mass = 0ull, larger = 0ull;
     unsigned count = 0;
@@ -567,7 +564,7 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
       const int lane = threadIdx.x & (MS_WAVE - 1);
       if (lane < n) {
         mine = w.candidates[lane];
-        mass = mass_of(key_value(mine), zmax);
+        mass = fixed_mass(key_value(mine), zmax);
       }
       for (int j = 0; j < n; ++j) {
         const unsigned key = __builtin_amdgcn_readlane(mine, j);
@@ -583,30 +580,30 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
       bool in = lane < n && (!a.k || count < (unsigned)a.k), ties_in = ties_in_k;
       unsigned long long kept_mass = sum(in ? mass : 0ull) + (ties_in ? tie_mass : 0ull);
       if (a.use_p) {
-        const double target = target_of(a.p, above_them ? whole : (double)kept_mass * MASS_UNIT);
-        known = above < target && above + (double)kept_mass * MASS_UNIT >= target;      // (it falls among the candidates)
-        ties_in = ties_in && (double)(kept_mass - tie_mass) * MASS_UNIT < target;
-        in = in && above + (double)larger * MASS_UNIT < target;
+        const unsigned long long target = target_of(a.p, above_them ? whole : kept_mass);
+        known = above < target && above + kept_mass >= target;      // (it falls among the candidates)
+        ties_in = ties_in && kept_mass - tie_mass < target;
+        in = in && above + larger < target;
         kept_mass = sum(in ? mass : 0ull) + (ties_in ? tie_mass : 0ull);
       }
       unsigned floor = in ? mine : 0xffffffffu;
       for (int o = MS_WAVE / 2; o > 0; o >>= 1) floor = min(floor, (unsigned)__shfl_xor((int)floor, o, MS_WAVE));
-      kept = Kept{ties_in ? min(floor, bound) : floor, above + (double)kept_mass * MASS_UNIT};
+      kept = Kept{ties_in ? min(floor, bound) : floor, above + kept_mass};
     } else if (known && !tied) {
       // many, and each of them itself: the descent over them (one row of 151,936 normal logits, top-p 0.9 at temperatures 0.7 and 3:
       // 41 and 45 us, compared with each other 58 and 100)
       const float s = (int)threadIdx.x < n ? key_value(w.candidates[threadIdx.x]) : NAN;
       kept = descend([&](auto f) { f(s); }, a.k, a.use_p, [&](unsigned long long total) -> unsigned long long {
         if (!above_them) return target_of(a.p, total);
-        const double need = ceil((target_of(a.p, whole) - above) / MASS_UNIT);
-        return need >= 1.0 && need <= (double)total ? (unsigned long long)need : 0ull;
+        const unsigned long long target = target_of(a.p, whole);
+        return target > above && target - above <= total ? target - above : 0ull;
       }, zmax, keys, masses, red);
-      known = kept.mass > 0.0;
+      known = kept.mass > 0ull;
       kept.mass += above;
     } else if (known) {
       if ((int)threadIdx.x < n) {
         mine = w.candidates[threadIdx.x];
-        mass = mass_of(key_value(mine), zmax);
+        mass = fixed_mass(key_value(mine), zmax);
         keys[threadIdx.x] = mine;
         masses[threadIdx.x] = mass;
       }
@@ -618,22 +615,23 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
       bool in = (int)threadIdx.x < n && (!a.k || count < (unsigned)a.k), ties_in = ties_in_k;
       unsigned long long kept_mass = block_sum_u64(in ? mass : 0ull, red) + (ties_in ? tie_mass : 0ull);
       if (a.use_p) {
-        const double target = target_of(a.p, (double)kept_mass * MASS_UNIT);
-        ties_in = ties_in && (double)(kept_mass - tie_mass) * MASS_UNIT < target;
-        in = in && (double)larger * MASS_UNIT < target;
+        const unsigned long long target = target_of(a.p, kept_mass);
+        ties_in = ties_in && kept_mass - tie_mass < target;
+        in = in && larger < target;
         kept_mass = block_sum_u64(in ? mass : 0ull, red) + (ties_in ? tie_mass : 0ull);
       }
       if (in) atomicMin(&floor_sm, mine);
       __syncthreads();
-      kept = Kept{ties_in ? min(floor_sm, bound) : floor_sm, (double)kept_mass * MASS_UNIT};
+      kept = Kept{ties_in ? min(floor_sm, bound) : floor_sm, kept_mass};
     }
     if (!known) {
       const int quads = (lead_of(row) + V + 3) / 4;
       kept = descend([&](auto f) { for_values(row, V, 0, quads, [&](float v) { f(v * a.inv_t); }); }, a.k, a.use_p,
                      [&](unsigned long long total) { return target_of(a.p, total); }, zmax, keys, masses, red);
     }
+    kept_sum = (double)kept.mass * MASS_UNIT;
   }
-  const float inv = (float)(1.0 / kept.mass), floor = kept.floor ? key_value(kept.floor) : -INFINITY;
+  const float inv = (float)(1.0 / kept_sum), floor = kept.floor ? key_value(kept.floor) : -INFINITY;
   for_quads(row, V, begin, end, [&](int i, const float4& v) {
     auto value = [&](float x) {
       const float s = x * a.inv_t;
@@ -661,6 +659,7 @@ extern "C" int ms_probabilities(const float* logits, long long ld, int n_rows, i
   // about two blocks a CU
   int n_chunks = (2 * ms_compute_units() + n_rows - 1) / n_rows;
   n_chunks = std::max(1, std::min(std::min(n_chunks, MAX_CHUNKS), (vocab + 2047) / 2048));
+  n_chunks = std::max(n_chunks, std::min((vocab - 1) / EXACT_SUMS + 1, MAX_CHUNKS));
   const dim3 grid(n_chunks, n_rows), block(THREADS);
   probabilities_max_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks);
   if (top_k || top_p) probabilities_collect_kernel<<<grid, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_k, top_p, work, n_chunks);

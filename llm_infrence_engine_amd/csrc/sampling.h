@@ -3,6 +3,11 @@
 #pragma once
 #include "common.h"
 
+// (for all that is behind this)  A scaled logit is rounded to a float before anything else is done with it: its key, its mass and its
+// probability are those of one number, wherever they are worked out (a product joined with the subtraction of the maximum is another
+// one), so that the kernels that choose and those that write distributions out keep the same tokens.
+#pragma clang fp contract(off)
+
 namespace {
 
 constexpr int THREADS = 1024;

@@ -475,6 +475,38 @@ def test_probabilities_are_what_sample_draws_from(T, k, p):
     assert ((often - M * w).abs() <= 5 * (M * w * (1 - w)).sqrt() + 1).all()
 
 
+@gpu
+@pytest.mark.parametrize("V,k", [(3000, 0), (3000, 500), (900, 0), (900, 300), (70001, 0)])
+def test_probabilities_keep_what_sample_keeps(V, k):
+    """Rows whose top-p lies, to 1e-10, where the mass of the largest tokens ends: whether the next one is kept hangs on how the
+    masses are rounded, so both have to take the same ones.  That token has a sixth of the kept mass: of 128 draws none has it, where
+    it is kept, once in 1e10."""
+    g = torch.Generator().manual_seed(V + k)
+    rows, draws = 24, 128
+    logits, p = torch.empty(rows, V), torch.empty(rows)
+    for r in range(rows):
+        x = -5.0 - math.log(V / 900) - 3.0 * torch.rand(V, generator=g)
+        large = torch.tensor([1.0, 0.8, 0.6, 0.5]) * (1 + 0.05 * torch.rand(4, generator=g))
+        x[[5, 200, 310, 777]] = large.sort(descending=True).values.log()
+        kept = x.sort(descending=True).indices[:k or V]
+        w = torch.exp(x.double())
+        before, total = w[[5, 200, 310]].sum(), w[kept].sum()
+        p[r] = before / total                       # a float: the mass of one small token is moved to where it is right
+        at = int(kept[20])
+        x[at] = torch.log(w[at] + before / p[r].double() - total).float()
+        logits[r] = x
+    many = logits.repeat_interleave(draws, 0).to(DEV)
+    M = rows * draws
+    T, ks, ps = torch.ones(M, device=DEV), ints([k] * M), p.repeat_interleave(draws).to(DEV)
+    out, drawn = torch.empty(rows, V, device=DEV), torch.empty(M, dtype=torch.int32, device=DEV)
+    ops.sample(many, drawn, T, ks, ps, torch.arange(M, dtype=torch.int64, device=DEV), torch.zeros(M, dtype=torch.int32, device=DEV))
+    ops.probabilities(logits.to(DEV), out, T[:rows].clone(), ks[:rows].clone(), p.to(DEV))
+    sampled = (drawn.view(rows, draws) == 777).any(1).cpu()
+    assert torch.isin(drawn, ints([5, 200, 310, 777])).all()
+    assert torch.equal((out[:, 777] > 0).cpu(), sampled)
+    assert (out > 0).sum(1).tolist() == [4 if s else 3 for s in sampled.tolist()]
+
+
 # ------------------------------------------------------------------------------------------------ verification
 def plain_verify(p, q, tokens, parents, starts, u, depth):
     """Request by request, the residual kept whole and normalised after every refusal (float64)."""
