@@ -30,7 +30,7 @@ constexpr int MAX_CHUNKS = 32, WAVES = THREADS / MS_WAVE;
 constexpr int MAX_CANDIDATES = THREADS;
 constexpr int BINS = 2048;
 constexpr float BINS_A_UNIT = 128.f;
-constexpr float NEAR_EDGE = 1.0f / 32768.f;      // of the whole mass; sums of up to 152,064 floats in any order are closer to their own
+constexpr float SUM_ERROR = 1.0f / 131072.f;     // of the histogram's sums, of the whole mass: some 60 additions of floats behind one another
 
 struct RowWork {                       // one per row, in the workspace the caller brings
   unsigned chunk_max[MAX_CHUNKS];      // key of the largest scaled logit of every chunk (no temperature: the largest itself)
@@ -74,8 +74,14 @@ __device__ __forceinline__ RowPlan plan_of(const float* temperature, const int* 
 // 4 q - lead .. + 3.
 __device__ __forceinline__ int lead_of(const float* row) { return (int)(((uintptr_t)row >> 2) & 3); }
 
+__device__ __forceinline__ int quads_of_chunk(const float* row, int V, int n_chunks) {
+  return ((lead_of(row) + V + 3) / 4 + n_chunks - 1) / n_chunks;
+}
+// Binary places of a mass in a chunk's histogram: as many as a bin of all of the chunk's values has room for.
+__device__ __forceinline__ int places_of(int quads) { return min(20, __builtin_clz(4 * max(1, quads)) - 1); }
+
 __device__ __forceinline__ void quad_range(const float* row, int V, int n_chunks, int c, int* begin, int* end) {
-  const int quads = (lead_of(row) + V + 3) / 4, len = (quads + n_chunks - 1) / n_chunks;
+  const int quads = (lead_of(row) + V + 3) / 4, len = quads_of_chunk(row, V, n_chunks);
   *begin = min(quads, c * len);
   *end = min(quads, *begin + len);
 }
@@ -344,9 +350,9 @@ probabilities_collect_kernel(const float* __restrict__ logits, size_t ld, int V,
   }
   double mine = 0.0;
   // In LDS a value adds to its bin, as a whole number, what its mass is of the mass at the bin's beginning, e^-f at f behind it (f <
-  // 1/128: 1 - f + f^2/2 is off by 2^-23); as many places as a bin of all of the chunk's values has room for.  Float additions in
-  // LDS took 5 times as long as whole ones (20 M values into 2,048 bins: 107 us, 23, the reading alone 23).
-  const int places = min(20, __builtin_clz(4 * max(1, end - begin)) - 1);
+  // 1/128: 1 - f + f^2/2 is off by 2^-23), rounded to the chunk's places.  Float additions in LDS took 5 times as long as whole ones
+  // (20 M values into 2,048 bins: 107 us, 23, the reading alone 23).
+  const int places = places_of(quads_of_chunk(row, V, n_chunks));
   const float whole = (float)(1 << places);
   for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0u;
   __syncthreads();
@@ -388,7 +394,11 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   const float zmax = key_value(largest_key(w, n_chunks));
   if (!finite(zmax)) return;
   const double whole = (double)sum_of(w.chunk_mass, n_chunks) * MASS_UNIT;
-  const float target = (float)((double)a.p * whole), near = (float)whole * NEAR_EDGE;
+  const float* row = logits + (size_t)r * ld;
+  // what the histogram may be off by: a mass by half a place of that at its bin's beginning, e^(1/128) times its own at most (2^-14
+  // where one chunk has 152,064 values), and the sums
+  const float half = 0.5f / (float)(1 << places_of(quads_of_chunk(row, V, n_chunks)));
+  const float target = (float)((double)a.p * whole), near = (float)whole * (half * (1.0f + 1.0f / 64.f) + SUM_ERROR);
   // the first bin at which the running mass reaches the target; a thread owns two bins
   const float h0 = w.hist[2 * threadIdx.x], h1 = w.hist[2 * threadIdx.x + 1];
   float run = h0 + h1;
@@ -412,7 +422,6 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   __syncthreads();
   const float high = zmax - (float)(found - up) * (1.0f / BINS_A_UNIT), low = zmax - (float)(found + 1 + down) * (1.0f / BINS_A_UNIT);
   if (c == 0 && threadIdx.x == 0) w.bin = found;
-  const float* row = logits + (size_t)r * ld;
   int begin, end;
   quad_range(row, V, n_chunks, c, &begin, &end);
   double above = 0.0;

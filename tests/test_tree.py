@@ -507,6 +507,25 @@ def test_probabilities_keep_what_sample_keeps(V, k):
     assert (out > 0).sum(1).tolist() == [4 if s else 3 for s in sampled.tolist()]
 
 
+@gpu
+def test_probabilities_of_many_rows_of_a_large_vocabulary():
+    """One block to a row, so that the histogram of a top-p alone has its fewest places, with masses that are all rounded the same
+    way among the rows; a k beyond what the groups of so few blocks are good for, and one within."""
+    g = torch.Generator().manual_seed(12)
+    V, M = 152064, 520
+    logits = 2.5 * torch.randn(4, V, generator=g)
+    logits[1] = (logits[1] * 100).round() / 100         # few different ones, hundreds of each
+    T, k, p = torch.tensor([0.9, 1.0, 1.1, 1.0]), ints([0, 0, 50, 20], "cpu"), torch.tensor([0.9, 0.7, 0.95, 1.0])
+    want = plain_probabilities(logits, T, k, p)
+    rows = torch.arange(M) % 4
+    many, out = logits.to(DEV)[rows.to(DEV)].contiguous(), torch.empty(M, V, device=DEV)
+    ops.probabilities(many, out, T[rows].to(DEV), k[rows].to(DEV), p[rows].to(DEV))
+    got = out[:4].cpu().double()
+    tiny = want < 1e-30
+    assert ((got > 0) == (want > 0))[~tiny].all() and ((got - want).abs() <= 2.8e-6 * want)[~tiny].all()
+    assert torch.equal(out, out[:4][rows.to(DEV)])
+
+
 # ------------------------------------------------------------------------------------------------ verification
 def plain_verify(p, q, tokens, parents, starts, u, depth):
     """Request by request, the residual kept whole and normalised after every refusal (float64)."""
