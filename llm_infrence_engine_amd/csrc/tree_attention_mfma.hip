@@ -810,7 +810,7 @@ extern "C" int ms_tree_attention_mfma_plan(int n_requests, int n_tokens, int max
     const double draws = tiles * context * head_dim * 4 / 13.5e6;
     for (const int n : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128}) {
       const long long share = ((context + n - 1) / n + turn - 1) / turn * turn, turns = share / turn, splits = (context + share - 1) / share;
-      if (splits > MAX_SPLITS) continue;
+      if (splits > MAX_SPLITS || share / 64 > 0xffff) continue;
       const double blocks = tiles * splits;
       const bool pairs = k.pair > 0.0 && blocks > cus;
       const double rounds = std::max(1.0, blocks / (pairs ? 2.0 * cus : cus));

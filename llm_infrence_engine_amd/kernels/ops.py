@@ -1668,18 +1668,27 @@ def tree_attention(q: torch.Tensor, kv, ctx, tree: torch.Tensor, out: torch.Tens
     d, page_size = kv.k_pages.shape[3], kv.k_pages.shape[2]
     dv = kv.v_pages.shape[2] if kv.v_transposed else kv.v_pages.shape[3]
     max_q_len, max_context_len = ctx.max_q_len, ctx.max_context_len
-    if q.shape[0] == 0 or ctx.context_lens.shape[0] == 0:
+    empty = q.shape[0] == 0 or ctx.context_lens.shape[0] == 0
+    if empty:
         max_q_len, max_context_len = max(1, max_q_len), max(1, max_context_len)
-    else:
-        _tree_bounds(max_q_len, max_context_len, kv.block_table, page_size)
     if q.dtype == torch.bfloat16:
         takes, per = kv.v_transposed and page_size % 16 == 0, 8
     else:
         takes, per = not kv.v_transposed and kv.k_pages.shape[0] * kv.k_pages.shape[1] * page_size < 1 << 31, 4
     if takes and d == dv and d in (32, 64, 128) and scale > 0 and (q.shape[0] == 1 or q.stride(0) % per == 0) and \
             (kv.k_pages.data_ptr() | kv.v_pages.data_ptr() | q.data_ptr() | out.data_ptr()) % 16 == 0:
-        return tree_attention_mfma(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.q_start, ctx.context_lens, tree, out,
-                                   num_heads, scale, max_q_len, max_context_len, kv.table_rows)
+        try:
+            return tree_attention_mfma(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.q_start, ctx.context_lens, tree, out,
+                                       num_heads, scale, max_q_len, max_context_len, kv.table_rows)
+        except UnsupportedShape:      # more tiles or keys than its grid takes
+            pass
+    if not empty:
+        _tree_bounds(max_q_len, max_context_len, kv.block_table, page_size)
+    if q.dtype == torch.bfloat16:
+        _say_once(("attention over trees", d, dv, page_size),
+                  f"bfloat16 attention over trees with keys of {d}, values of {dv} and pages of {page_size} tokens runs on the vector-ALU "
+                  f"kernel: the matrix-core kernel takes keys and values of 32, 64 and 128, value pages transposed, pages of a multiple of "
+                  f"16, rows on 16 bytes and up to 65,535 tiles")
     return tree_attention_generic(q, kv.k_pages, kv.v_pages, kv.block_table, ctx.token_req, ctx.q_start, ctx.context_lens, tree,
                                   out, num_heads, scale, max_q_len, kv.v_transposed, kv.table_rows, ctx.n_live_tokens)
 

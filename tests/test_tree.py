@@ -1210,6 +1210,36 @@ def test_tree_attention_refuses_views_with_a_window_or_entries_of_several_tokens
     assert len(host) == 1
 
 
+def test_steps_that_the_matrix_kernel_has_no_room_for_go_to_the_other(host, monkeypatch):
+    """Sizes that its plan, or its launch, does not take are the vector kernel's; what is wrong for either is refused."""
+    monkeypatch.setattr(ops, "_get", lambda name: lambda *a: 0)
+    tree_call(32)
+    assert host == ["ms_tree_attention_generic"]
+    monkeypatch.setattr(ops, "_get", lambda name: lambda *a: 64)
+    call = ops._call
+
+    def no_room(name, *a):
+        if name == "ms_tree_attention_f32":
+            raise ops.UnsupportedShape(name)
+        call(name, *a)
+
+    monkeypatch.setattr(ops, "_call", no_room)
+    tree_call(32)
+    assert host == ["ms_tree_attention_generic"] * 2
+    del host[:]
+    refused(host, lambda: tree_call(32, max_context_len=9))
+
+
+def test_the_plan_of_the_longest_contexts_fits_its_number():
+    """Up to its last bound of keys the plan names a kind there is and a share of them, for few blocks as for many."""
+    for R, N, nh, nkv, d in ((1, 1, 14, 2, 64), (512, 512, 14, 2, 64), (65535, 65535, 32, 8, 128), (1024, 4096, 32, 1, 128)):
+        for keys in (64, 64 * 65534, 64 * 65535):
+            plan = ops._get("ms_tree_attention_mfma_plan")(R, N, 1 if N == R else 8, keys, nh, nkv, d, 16)
+            share = (plan & 0xFFFF) * 64
+            assert 0 <= plan >> 16 < 4 and share > 0 and -(-keys // share) <= 128
+        assert ops._get("ms_tree_attention_mfma_plan")(R, N, 1, 64 * 65535 + 1, nh, nkv, d, 16) == -1
+
+
 def test_pools_that_cannot_drop_tokens_refuse(host):
     from llm_infrence_engine_amd.cache.pools import CachePools
 
