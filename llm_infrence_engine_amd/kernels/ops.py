@@ -1743,7 +1743,9 @@ def keep_tokens(pages, transposed, block_table: torch.Tensor, first: torch.Tenso
     i < counts[r], in every layer and head of every tensor of ``pages``: [layers, pages, heads, page_size, width] each, or
     [layers, pages, heads, width, page_size] where ``transposed`` says so (or without the layers).  ``first`` int32 [R]: the
     entry of the step's first token (context length less tokens); ``nodes`` int32 [R, depth] and ``counts`` int32 [R] as
-    ``verify_drafts`` leaves them: increasing, 0 first.  Entries whose page is the null page or outside the pool stay."""
+    ``verify_drafts`` leaves them: increasing, 0 first.  Entries whose page is the null page or outside the pool stay.  All of a
+    call is moved at once: the page tensors are other memory each, and no two requests have the same row or share a page that one
+    of them moves entries to."""
     n = len(pages)
     if n == 0 or n != len(transposed):
         raise ValueError("one or more page tensors, and for each whether it is transposed")
@@ -1776,8 +1778,9 @@ def keep_tokens(pages, transposed, block_table: torch.Tensor, first: torch.Tenso
         elif sizes != (L, P, page_size):
             raise ValueError("the page tensors of a call have the same layers, pages and page size")
         record += _KEPT_TENSOR.pack(t.data_ptr(), heads, width, bool(flip), 0)
-    if len({t.data_ptr() for t in pages}) != n:
-        raise ValueError("a page tensor stands in the call twice")
+    places = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in pages)
+    if any(end > begin for (_, end), (begin, _) in zip(places, places[1:])):
+        raise ValueError("page tensors of a call must not share memory (one stands in it twice?)")
     if R == 0 or depth == 0 or 0 in pages[0].shape:
         return
     if R > 65535:

@@ -1240,6 +1240,20 @@ def test_the_plan_of_the_longest_contexts_fits_its_number():
         assert ops._get("ms_tree_attention_mfma_plan")(R, N, 1, 64 * 65535 + 1, nh, nkv, d, 16) == -1
 
 
+def test_keep_tokens_refuses_page_tensors_that_share_memory(host):
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32)     # noqa: E731
+    call = lambda *pages: ops.keep_tokens(list(pages), [False] * len(pages), z(4, 5), z(2), z(2, 3), z(2), z(2))     # noqa: E731
+    pool = torch.zeros(3, 7, 2, 16, 8)
+    other = torch.zeros(2, 7, 2, 16, 8)
+    refused(host, lambda: call(pool[:2], pool[1:]))
+    refused(host, lambda: call(pool[1:], other, pool[:2]))
+    refused(host, lambda: call(pool, pool))
+    refused(host, lambda: call(other, other.view(-1).view(2, 7, 2, 16, 8)))
+    call(pool[0], pool[1], pool[2])
+    call(pool[:2], other)
+    assert host == ["ms_keep_tokens"] * 2
+
+
 def test_pools_that_cannot_drop_tokens_refuse(host):
     from llm_infrence_engine_amd.cache.pools import CachePools
 
