@@ -323,6 +323,97 @@ def test_tree_attention_of_infinite_values(monkeypatch, dtype, bad, nh, nkv, d):
                 assert (got[n] == bad).all() if hit else torch.isfinite(got[n]).all(), (share, at, n)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (2, 1, 128), (4, 2, 32)])
+def test_tree_attention_of_more_than_64_shares(monkeypatch, dtype, nh, nkv, d):
+    """The join has a second part for a lane from the 65th share on; what stands in those decides the result: the step's own values
+    are a hundred times the others.  The two parts with their sums are floats: nothing on top of ``close_enough``."""
+    get = ops._get
+    for share in (128, 192):
+        forced = {"ms_tree_attention_mfma_plan": 65536 + share // 64, "ms_tree_attention_f32_share": share}
+        monkeypatch.setattr(ops, "_get", lambda name: (lambda *a: forced[name]) if name in forced else get(name))
+        s = make_step(dtype, nh, nkv, d, 16, [3, 1, 7], [12500, 70 * share + 5, 8400], seed=8)
+        for r in range(3):
+            for at in range(s.contexts[r] - s.trees[r], s.contexts[r]):
+                page, slot = int(s.kv.block_table[s.kv.table_rows[r], at // 16]), at % 16
+                s.V[r][:, at] *= 100
+                value = s.V[r][:, at].to(DEV)
+                if s.kv.v_transposed:
+                    s.kv.v_pages[page, :, :, slot] = value
+                else:
+                    s.kv.v_pages[page, :, slot] = value
+        ops.tree_attention(s.q, s.kv, s.ctx, s.tree, s.out, s.nh, s.scale)
+        close_enough(s)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (8, 2, 128), (4, 2, 32), (6, 1, 20)])
+def test_tree_attention_of_a_key_that_is_nan(dtype, nh, nkv, d):
+    """A token that sees it gets NaN throughout, one that does not what it gets without."""
+    trees, contexts = [37, 9], [300, 9]
+    sees = [ancestors(random_tree(random.Random(4), n)) for n in trees]
+    s = make_step(dtype, nh, nkv, d, 16, trees, contexts, seed=6, sees=sees)
+    at = contexts[0] - trees[0] + 11
+    s.kv.k_pages[int(s.kv.block_table[s.kv.table_rows[0], at // 16]), :, at % 16] = math.nan
+    ops.tree_attention(s.q, s.kv, s.ctx, s.tree, s.out, s.nh, s.scale)
+    for n, row in enumerate(s.out.cpu()):
+        hit = n < 37 and 11 in sees[0][n]
+        assert torch.isnan(row).all() if hit else torch.isfinite(row).all(), n
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (8, 2, 128), (5, 1, 48)])
+def test_tree_attention_replayed_with_the_bounds_of_a_cache(dtype, nh, nkv, d):
+    """A captured step's bounds are its batch's tokens and the cache's capacity; contexts, trees and the count of live tokens change
+    between the replays, each checked against 64 bits and against the eager call."""
+    s = make_step(dtype, nh, nkv, d, 16, [8, 5, 13], [300, 40, 2000], seed=1)
+    N, R = 32, 3
+    table = torch.zeros(s.kv.block_table.shape[0], 2048, dtype=torch.int32, device=DEV)
+    table[:, :s.kv.block_table.shape[1]] = s.kv.block_table
+    s.kv.block_table = table
+    s.ctx.max_q_len, s.ctx.max_context_len = N, 32768
+    q, out = torch.zeros(N, nh * d, dtype=dtype, device=DEV), torch.zeros(N, nh * d, dtype=dtype, device=DEV)
+    tree, s.ctx.n_live_tokens = torch.zeros(N, 1, dtype=torch.int32, device=DEV), ints([26])
+    s.ctx.token_req, s.ctx.q_start, s.ctx.context_lens = ints([0] * N), ints([0] * (R + 1)), ints([0] * R)
+    q[:26] = s.q
+
+    def step():
+        ops.tree_attention(q, s.kv, s.ctx, tree, out, nh, s.scale)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.inference_mode(), torch.cuda.graph(graph, stream=side):
+        step()
+    for trees, contexts in (([8, 5, 13], [300, 40, 2000]), ([1, 0, 25], [7, 0, 1999]), ([10, 1, 2], [10, 33, 64]), ([0, 0, 0], [0, 0, 0])):
+        sees = [ancestors(random_tree(random.Random(n), n)[:n]) for n in trees]
+        starts = [0, trees[0], trees[0] + trees[1], sum(trees)]
+        live = starts[-1]
+        s.ctx.token_req.copy_(ints([r for r, n in enumerate(trees) for _ in range(n)] + [0] * (N - live)))
+        s.ctx.q_start.copy_(ints(starts))
+        s.ctx.context_lens.copy_(ints(contexts))
+        s.ctx.n_live_tokens.copy_(ints([live]))
+        tree.zero_()
+        if live:
+            tree[:live] = ints([w for x in sees for w in mask_words(x, 1)])
+        both = []
+        for run in (graph.replay, step):
+            out.fill_(3.0)
+            run()
+            torch.cuda.synchronize()
+            both.append(out.clone())
+        assert torch.equal(*both) and (out[live:] == 3.0).all()
+        now = SimpleNamespace(**{**vars(s), "trees": trees, "contexts": contexts, "sees": sees, "starts": starts, "q": q[:live], "out": out[:live]})
+        if live:
+            close_enough(now)
+
+
 # ------------------------------------------------------------------------------------------------ probabilities
 def plain_probabilities(logits, T, top_k, top_p):
     """float64, row by row; the scaled logits are floats, as the sampler has them."""
