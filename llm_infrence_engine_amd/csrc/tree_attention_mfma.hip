@@ -602,18 +602,20 @@ tree_attention_f32_kernel(const float* __restrict__ q, size_t q_stride, const fl
       if (t + 2 * F32_WAVES < t_end) row_next = row_of(t + 2 * F32_WAVES);
     }
     const int base = t * 16;
-    f32x4 s[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // a score is summed in four parts: the rounding of the longer chain of one made results off by up to 2.2 times what a plain
+    // product in float is (now 1.1; 120 steps of up to 16 tokens behind up to 600 keys)
+    f32x4 s[NT], quarter[NT][4] = {};
 #pragma unroll
     for (int j = 0; j < CT; ++j)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].x, qv[n][j].x, s[n], 0, 0, 0);
-        s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].y, qv[n][j].y, s[n], 0, 0, 0);
-        s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].z, qv[n][j].z, s[n], 0, 0, 0);
-        s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].w, qv[n][j].w, s[n], 0, 0, 0);
+        quarter[n][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].x, qv[n][j].x, quarter[n][0], 0, 0, 0);
+        quarter[n][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].y, qv[n][j].y, quarter[n][1], 0, 0, 0);
+        quarter[n][2] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].z, qv[n][j].z, quarter[n][2], 0, 0, 0);
+        quarter[n][3] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].w, qv[n][j].w, quarter[n][3], 0, 0, 0);
       }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n] = (quarter[n][0] + quarter[n][1]) + (quarter[n][2] + quarter[n][3]);
     const bool masked = base + 16 > before;
     unsigned sees[NT];
     bool spoiled = false;

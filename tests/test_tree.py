@@ -297,6 +297,20 @@ def test_tree_attention_weights_are_not_rounded_to_bfloat16(monkeypatch, nh, nkv
 
 
 @gpu
+@pytest.mark.parametrize("trees,contexts", [([7, 4], [49, 60]), ([2, 3, 5], [34, 48, 60])])
+def test_tree_attention_sums_scores_of_floats_in_short_chains(trees, contexts):
+    """Roundings that are independent of each other, each half a step over sqrt(3): a score of 128 dims in four chains of 32 sums of up
+    to 8 (half a step 2.4e-7) is off by 2.4e-7 / sqrt(3) * sqrt(128) * 0.6 = 9.4e-7, times the scale 0.8e-7; the exponent, up to 8 in
+    powers of two, by 1e-7; the exponential 0.7e-7, sums and quotient 0.6e-7: 1.6e-7 together, of a weight and so of a result of
+    random values.  Twice that is allowed; one chain of 128 sums of up to 16 had 4.5e-7."""
+    s = make_step(F32, 8, 2, 128, 16, trees, contexts, seed=3)
+    ops.tree_attention(s.q, s.kv, s.ctx, s.tree, s.out, s.nh, s.scale)
+    want, _ = plain_attention(s)
+    off = (s.out.cpu().double().view(want.shape) - want).norm() / want.norm()
+    assert off <= 3.2e-7, off
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("bad", [math.inf, -math.inf])
 @pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (8, 2, 128), (4, 2, 32), (6, 1, 20)])
