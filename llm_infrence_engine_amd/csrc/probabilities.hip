@@ -385,7 +385,7 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
                           const int* __restrict__ top_k, const float* __restrict__ top_p, RowWork* __restrict__ work, int n_chunks) {
   __shared__ unsigned long long red[WAVES];
   __shared__ float wave_sum_sm[WAVES];
-  __shared__ int found, up, down;      // the target's bin; those before and behind it that count too
+  __shared__ int found, up, down;      // the target's bin; the first and the last that count
   __shared__ Candidates here;
   const int r = blockIdx.y, c = blockIdx.x, lane = threadIdx.x & (MS_WAVE - 1), wave = threadIdx.x / MS_WAVE;
   RowWork& w = work[r];
@@ -416,11 +416,25 @@ probabilities_near_kernel(const float* __restrict__ logits, size_t ld, int V, co
   if (found >= BINS) return;
   if (found >> 1 == (int)threadIdx.x) {
     const float upto = found & 1 ? run : run - h1, from = upto - (found & 1 ? h1 : h0);
-    up = target - from < near;
-    down = upto - target < near;
+    up = target - from < near ? -1 : found;
+    down = upto - target < near ? BINS : found;
   }
   __syncthreads();
-  const float high = zmax - (float)(found - up) * (1.0f / BINS_A_UNIT), low = zmax - (float)(found + 1 + down) * (1.0f / BINS_A_UNIT);
+  if (up < 0 || down == BINS) {
+    // a neighbour is the next bin that holds anything: where few tokens have most of the mass, many between them are empty
+    const bool before = up < 0, behind = down == BINS;
+    __syncthreads();
+    if (before && h0 + h1 > 0.f) {
+      if (h1 > 0.f && 2 * (int)threadIdx.x + 1 < found) atomicMax(&up, 2 * (int)threadIdx.x + 1);
+      else if (h0 > 0.f && 2 * (int)threadIdx.x < found) atomicMax(&up, 2 * (int)threadIdx.x);
+    }
+    if (behind && h0 + h1 > 0.f) {
+      if (h0 > 0.f && 2 * (int)threadIdx.x > found) atomicMin(&down, 2 * (int)threadIdx.x);
+      else if (h1 > 0.f && 2 * (int)threadIdx.x + 1 > found) atomicMin(&down, 2 * (int)threadIdx.x + 1);
+    }
+    __syncthreads();
+  }
+  const float high = zmax - (float)up * (1.0f / BINS_A_UNIT), low = zmax - (float)(min(down, BINS - 1) + 1) * (1.0f / BINS_A_UNIT);
   if (c == 0 && threadIdx.x == 0) w.bin = found;
   int begin, end;
   quad_range(row, V, n_chunks, c, &begin, &end);
