@@ -377,7 +377,7 @@ verify_drafts_kernel(const float* __restrict__ p, const float* __restrict__ q, i
 // A block works a request's moves out once (where they lie: table and pages) and its waves then walk (layer, head) pairs of one
 // tensor; where each thread did it for itself it waited for path, table and entry one after another (32 requests, 64 layers of 8
 // heads of 128 in bfloat16: 98 us).  In transposed pages an entry is one value of every row, so what has to be read and written
-// is all lines of its page's part of a head: 190 MB for those 75, 41 us as a copy takes them.  There a wave reads a row's 32 bytes
+// is all lines of its page's part of a head: 184 MB read and 102 written for those 75, 61 us as a copy takes them.  There a wave reads a row's 32 bytes
 // around the moves' places, puts the values in and writes the 32 bytes back, whole lines for memory (68 us; value by value 74).
 struct KeepTensor {
   void* pages;

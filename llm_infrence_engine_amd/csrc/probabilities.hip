@@ -17,8 +17,9 @@
 //     candidates a radix descent over their keys finds it); then every block writes its chunk
 // What the candidates cannot decide (more than MAX_CANDIDATES of them, a k beyond half the groups, a target outside the
 // candidates' masses) every block of the row finds by itself with a radix descent over the whole row: right for any input, and
-// slow (a row of 151,936: 110 us for a k of half of them, 190 for top-p 0.5 of normal logits at a temperature of 3, 360 where all are
-// alike; 26 to 43 otherwise).
+// slow (a row of 151,936: 105 us for a k of half of them, 190 for top-p 0.5 of normal logits at a temperature of 3, 360 where all are
+// alike; 25 to 38 otherwise).  Half the groups are 32 to a block at most, and a row has 512 / rows blocks, rounded up: k up to 64 with
+// 256 rows, 32 with 512 (151,936, top-k 50, top-p 0.9: 140 us with 256 rows, 580 with 512).
 #include "sampling.h"
 #include "api.h"
 #include <algorithm>
@@ -614,7 +615,7 @@ probabilities_write_kernel(const float* __restrict__ logits, size_t ld, int V, c
       kept = Kept{ties_in ? min(floor, bound) : floor, above + kept_mass};
     } else if (known && !tied) {
       // many, and each of them itself: the descent over them (one row of 151,936 normal logits, top-p 0.9 at temperatures 0.7 and 3:
-      // 41 and 45 us, compared with each other 58 and 100)
+      // 36 and 38 us; when they took 41 and 45, compared with each other 58 and 100)
       const float s = (int)threadIdx.x < n ? key_value(w.candidates[threadIdx.x]) : NAN;
       kept = descend([&](auto f) { f(s); }, a.k, a.use_p, [&](unsigned long long total) -> unsigned long long {
         if (!above_them) return target_of(a.p, total);

@@ -10,7 +10,8 @@
 // Scores, maximum, exponentials, their sum and the weighted sum of values are float.
 // This is the kernel of the sizes and layouts that csrc/tree_attention_mfma.hip does not take: a block owns one
 // (token, query head), its waves take blocks of 64 keys in turn (a lane reads its own key's row, then every lane its own
-// entries of one row of values after another) and are merged through LDS in order.
+// entries of one row of values after another) and are merged through LDS in order.  Every key is read for every token and head:
+// 8 trees of up to 16 behind up to 2,000 keys, 28 heads of 48 on 4 in bfloat16, 465 us.
 #include "common.h"
 #include "api.h"
 

@@ -505,7 +505,7 @@ tree_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ 
 // quarters of 16 dims, and one of the value product one key of each of four quarters of 16, so that a lane reads 16 bytes of its
 // key's row and has its own keys' weights where they are: O^T[dim, col] += V^T[dim, key] . P^T[key, col].  Pages may have any size.
 // 157 TFLOP/s are more than it can be fed: it waits for its loads (6 trees of up to 13 tokens behind 700 keys, 14 heads of 64 on 2:
-// 60 us on the vector ALUs, which read every key for every column).
+// 9 us, 60 on the vector ALUs, which read every key for every column).
 constexpr int F32_WAVES = 8;
 
 template <int D, int NT>
