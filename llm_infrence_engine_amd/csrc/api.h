@@ -245,7 +245,8 @@ int ms_probabilities(const float* logits, long long ld, int n_rows, int vocab, c
 
 // ---- steps that check trees of drafted tokens (csrc/tree_attention.hip, csrc/drafts.hip).
 // Token n, the i-th of request r = token_req[n], sees the entries of r before the step's and of the step's entries those with
-// a bit in its row of tree int32 [n_tokens, words].  context_lens [R]: entries with the step's.
+// a bit in its row of tree int32 [n_tokens, words].  context_lens [R]: entries with the step's.  max_q_len and max_context_len are upper
+// bounds: what lies behind them is not looked at.
 int ms_tree_attention_generic(const void* q, long long q_stride, const void* k_pages, const void* v_pages, const int* block_table,
                               int table_stride, const int* table_rows, const int* token_req, const int* q_start,
                               const int* context_lens, const int* n_live_tokens, const int* tree, int words, void* out,
@@ -282,7 +283,8 @@ long long ms_verify_drafts_workspace_bytes(int n_requests);      // of workspace
 void ms_verify_drafts_patience(int looks);                       // tests
 
 // tensors: in host memory n_tensors (at most ms_keep_tokens_max()) of {void* pages; int heads, width, transposed, 0}, pages
-// [layers, num_pages, heads, page_size, width] or [.., width, page_size].  Entry first[r] + nodes[r][i] goes to first[r] + i.
+// [layers, num_pages, heads, page_size, width] or [.., width, page_size], no memory in two of them.  Entry first[r] + nodes[r][i]
+// goes to first[r] + i; no two requests have the same table row.
 int ms_keep_tokens_max();
 int ms_keep_tokens(const void* tensors, int n_tensors, int layers, int num_pages, int page_size, const int* block_table,
                    int table_stride, const int* table_rows, const int* first, const int* nodes, int depth, const int* counts,

@@ -133,7 +133,7 @@ __device__ __forceinline__ float exp_of(float x) {
 __device__ __forceinline__ double whole_mass(float s, float zmax) {
   return (double)truncf(expf(fmaxf(s - zmax, -200.f)) * (float)(1ull << FIX_PLACES));
 }
-constexpr int EXACT_SUMS = 512 * THREADS;      // values a chunk
+constexpr int EXACT_SUMS = 504 * THREADS;      // values a chunk: a thread has four more of an uneven share, and four of a row's end
 constexpr double MASS_UNIT = 1.0 / (double)(1ull << FIX_PLACES);
 
 __device__ double block_sum_double(double v, double* red) {
